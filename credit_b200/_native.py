@@ -25,6 +25,8 @@ F32 = 0
 BF16 = 1
 COMM_ID_BYTES = 128      # credit_comm_get_unique_id
 PEER_HANDLE_BYTES = 64   # credit_peer_group_create
+MAX_TOP = 128            # alternatives, and a teacher's list
+STATUS_WAIT_TIMEOUT, STATUS_BAD_GEOMETRY, STATUS_BAD_INDEX = 1, 2, 4   # bits of device_status()
 
 VARIANT_AUTO, VARIANT_BLOCK_READ, VARIANT_BLOCK_SMEM, VARIANT_CLUSTER_SMEM = 0, 1, 2, 3
 LOAD_AUTO, LOAD_TMA, LOAD_LDG = 0, 1, 2
@@ -176,6 +178,23 @@ PROTOTYPES: dict[str, tuple] = {
     "credit_ffn_forward_host": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_float, c_void_p,
                 c_size_t, c_void_p]),
+    "credit_residual_norm_forward": (
+        c_int, [c_void_p] * 9 + [c_int64, c_int64, c_float, c_float, c_int, _OPTS_P, c_void_p]),
+    "credit_residual_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int, _OPTS_P]),
+    "credit_residual_norm_backward": (
+        c_int, [c_void_p] * 14 + [c_int64, c_int64, c_float, c_int, _OPTS_P, c_void_p, c_size_t, c_void_p]),
+    "credit_token_logprobs_forward": (
+        c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64,
+                c_float, c_int, _OPTS_P, c_void_p]),
+    "credit_token_logprobs_backward": (
+        c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                c_float, c_int, _OPTS_P, c_void_p]),
+    "credit_distill_topk_forward": (
+        c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_float, c_int,
+                c_int, _OPTS_P, c_void_p]),
+    "credit_distill_topk_backward": (
+        c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                c_float, c_int, _OPTS_P, c_void_p]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,523 @@
+// Distillation from a teacher's top logits: KL(teacher || student) per row, where the teacher is a
+// list of up to 128 columns with log probabilities, and its gradient with respect to the student's
+// logits. With z = logits / temperature, q = softmax(z), list entries k with column c_k:
+//   without a tail  w_k = softmax(v)_k              (the teacher renormalised over its list)
+//   with a tail     w_k = exp(v_k), w_r = 1 - sum w_k against q_r = sum of q outside the list
+//   loss = sum_k w_k (log w_k - log q_{c_k}) [+ w_r (log w_r - log q_r)]
+//   dlogits_j = g / temperature * (q_j - w_j)                      for j in the list
+//             = g / temperature * exp(z_j - tail lse) (q_r - w_r)  outside it (q_j without a tail)
+// The sum outside the list is accumulated as such (listed columns are marked in a bitmap and skipped),
+// never as "all minus listed", so a student that has almost all of its mass in the list keeps q_r and
+// its gradient to full precision; w_r is taken in 64 bits for the same reason.
+// No reference kernel exists for this; the row pass is that of token_logprobs.cu.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+
+#include "device_context.h"
+#include "vocab_host.h"
+#include "vocab_rows.cuh"
+
+namespace credit {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;
+constexpr int kMaxList = 128;
+constexpr int kPerLane = kMaxList / 32;
+constexpr int kStats = 6;   // floats of saved state per row
+
+struct DistillArgs {
+    const void* logits;
+    int64_t ld;
+    const int64_t* index;    // [rows, top_k], negative = unused place
+    const float* teacher;    // [rows, top_k]
+    int top_k;
+    float* loss;
+    float* stats;            // [rows, 6]
+    int cols;
+    int slice;
+    int bitmap_words;        // of one slice
+    float inv_t;
+    int* status;
+};
+
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// One row's list in shared memory.
+struct TeacherList {
+    int column[kMaxList];      // -1 = unused
+    float value[kMaxList];
+    double mass;               // tail: sum of exp(value); no tail: of exp(value - log_norm) (1, or 0 for none)
+    float log_norm;            // no tail: log sum exp(value)
+    int bad;                   // some column lies outside the row
+    int any;                   // some place is used
+};
+
+// Warp 0 reads the list; all threads see it behind a barrier that the caller places.
+template <bool TAIL>
+__device__ __forceinline__ void load_list(const DistillArgs& a, int64_t row, TeacherList& l) {
+    if (threadIdx.x >= 32) return;
+    const int lane = threadIdx.x;
+    float v[kPerLane];
+    bool bad = false, any = false;
+    float top = -CUDART_INF_F;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        const int k = lane + 32 * i;
+        int column = -1;
+        v[i] = -CUDART_INF_F;
+        if (k < a.top_k) {
+            const int64_t c = a.index[row * a.top_k + k];
+            if (c >= a.cols) {
+                bad = true;
+            } else if (c >= 0) {
+                column = static_cast<int>(c);
+                v[i] = a.teacher[row * a.top_k + k];
+                any = true;
+            }
+        }
+        l.column[k] = column;
+        l.value[k] = v[i];
+        top = max_nan(top, v[i]);
+    }
+    top = warp_max_nan(top);
+    const float base = TAIL || top == -CUDART_INF_F ? 0.0f : top;
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) sum += exp(static_cast<double>(v[i]) - base);
+    sum = warp_sum_f64(sum);
+    bad = __any_sync(0xffffffffu, bad);
+    any = __any_sync(0xffffffffu, any);
+    if (lane == 0) {
+        l.log_norm = TAIL || sum == 0.0 ? 0.0f : static_cast<float>(base + log(sum));
+        l.mass = TAIL ? sum : (sum == 0.0 ? 0.0 : 1.0);
+        l.bad = bad;
+        l.any = any;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// forward: one cluster per row, the row read once
+// ---------------------------------------------------------------------------
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(kThreads) distill_topk_kernel(const DistillArgs a) {
+    __shared__ SoftmaxRecord warp_records[kThreads / 32];
+    __shared__ SoftmaxRecord records[kMaxClusterSize];
+    __shared__ TeacherList list;
+    extern __shared__ __align__(16) uint32_t bitmap[];   // TAIL: one bit per element of the slice, vectors first
+
+    constexpr int E = Vec<T>::kElems;
+    const uint32_t rank = cluster_cta_rank(), nranks = cluster_cta_count();
+    const int64_t row = blockIdx.x / nranks;
+    const int tid = threadIdx.x;
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    const int start = static_cast<int>(rank) * a.slice;
+    const int local = max(0, min(a.slice, a.cols - start));
+    const RowSpan<T> span(x, start, local);
+    const float k2 = a.inv_t * kLog2e;
+
+    load_list<TAIL>(a, row, list);
+    if (TAIL)
+        for (int i = tid; i < a.bitmap_words; i += kThreads) bitmap[i] = 0;
+    __syncthreads();
+    if (!list.bad && (TAIL ? !list.any : list.mass == 0.0)) {
+        // no teacher in this row: nothing is read (the whole cluster leaves here)
+        if (rank == 0) {
+            if (tid == 0) a.loss[row] = 0.0f;
+            if (tid < kStats) a.stats[row * kStats + tid] = tid == 0 ? -CUDART_INF_F : 0.0f;   // no gradient
+        }
+        return;
+    }
+    cluster_arrive_release();
+    // bit of an element: its place in the vectors, or behind them for the edges
+    auto place_of = [&](int offset) {
+        const int v = offset - span.head;
+        if (v >= 0 && v < span.nvec * E) return v;
+        return span.nvec * E + (offset < span.head ? offset : offset - span.nvec * E);
+    };
+    float listed = -CUDART_INF_F;   // the student's logit at list entry tid, for the row's finish in rank 0
+    if (tid < a.top_k && list.column[tid] >= 0) {
+        const int offset = list.column[tid] - start;
+        if (TAIL && offset >= 0 && offset < local) {
+            const int p = place_of(offset);
+            atomicOr(&bitmap[p >> 5], 1u << (p & 31));
+        }
+        if (rank == 0) listed = Vec<T>::load(x + list.column[tid]);
+    }
+    if (TAIL) __syncthreads();
+
+    SoftmaxRecord rec = empty_record();
+    auto add = [&](auto& v) {
+        constexpr int U = sizeof(v) / sizeof(uint4);
+        float part[U];
+        const float top = chunk_max<T, U>(v, part);
+        accumulate<T, U, false>(v, top, k2, rec);
+    };
+    // listed elements of a vector become masked ones
+    auto hide = [&](uint4& v, uint32_t bits) {
+        float y[E];
+        Vec<T>::unpack(v, y);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (bits >> j & 1u) y[j] = -CUDART_INF_F;
+        v = Vec<T>::pack(y);
+    };
+    stream_slice<T, kThreads, kUnroll>(
+        span,
+        [&](uint4 (&v)[kUnroll], int first, int) {
+            if (TAIL) {
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    const int p = (first + u * kThreads) * E;
+                    const uint32_t bits = p < span.nvec * E ? bitmap[p >> 5] >> (p & 31) & ((1u << E) - 1u) : 0u;
+                    if (bits != 0) hide(v[u], bits);
+                }
+            }
+            add(v);
+        },
+        [&](uint4 (&v)[1]) {
+            if (TAIL && tid < span.edges) {
+                const int p = span.nvec * E + tid;
+                if (bitmap[p >> 5] >> (p & 31) & 1u) v[0] = masked_vec<T>();
+            }
+            add(v);
+        });
+    rec = cta_record<kThreads>(rec, warp_records, k2);
+    cluster_wait_acquire();
+    if (nranks > 1) {
+        if (rank != 0 && tid == 0) {
+            const uint32_t to = map_to_rank(smem_u32(&records[rank]), 0);
+            st_cluster_f32(to, rec.m);
+            st_cluster_f32(to + 4, rec.s);
+            st_cluster_f32(to + 8, rec.e);
+        }
+        cluster_sync_all();
+        if (rank != 0) return;
+    }
+    // rank 0, warp 0 finishes the row; lane l holds list entries l, l + 32, ... (their logits come
+    // through shared memory)
+    __shared__ float student[kMaxList];
+    if (tid < kMaxList) student[tid] = listed;
+    __syncthreads();
+    if (tid >= 32) return;
+    for (uint32_t r = 1; r < nranks; ++r) rec = merge_records(rec, records[r], k2);
+    SoftmaxRecord all = rec;   // with a tail `rec` covers the columns outside the list
+    if (TAIL) {
+        // the listed columns, each once: a repeated column counts where it appears first
+        float y[kPerLane];
+        float top = -CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) {
+            const int k = tid + 32 * i;
+            const int c = list.column[k];
+            bool repeated = false;
+            for (int j = 0; j < k; ++j) repeated |= list.column[j] == c;
+            y[i] = c < 0 || repeated ? -CUDART_INF_F : student[k];
+            top = max_nan(top, y[i]);
+        }
+        SoftmaxRecord mine = empty_record();
+        mine.m = warp_max_nan(top);
+        const float base = mine.m == -CUDART_INF_F ? 0.0f : mine.m;
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i) mine.s += ex2_approx((y[i] - base) * k2);
+        mine.s = warp_sum(mine.s);
+        all = merge_records(rec, mine, k2);
+    }
+    const bool broken = is_broken(all.m) || list.bad;
+    const bool empty = all.m == -CUDART_INF_F, no_tail = rec.m == -CUDART_INF_F;
+    const float log_sum = empty ? 0.0f : logf(all.s);
+    const float tail_log_sum = no_tail ? 0.0f : logf(rec.s);
+    // the teacher: always a distribution. Without anything left outside the student's list, or with a
+    // list of more than 1, it is renormalised over the list.
+    float log_norm = list.log_norm, rest = 0.0f;
+    bool no_teacher = false;
+    if (TAIL) {
+        const double left = 1.0 - list.mass;
+        if (no_tail || left < 0.0) {
+            no_teacher = list.mass == 0.0;   // all of it outside the list, and nothing is there
+            log_norm = no_teacher ? 0.0f : static_cast<float>(log(list.mass));
+        } else {
+            rest = static_cast<float>(left);
+        }
+    }
+    double loss = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+        const int k = tid + 32 * i;
+        const float logw = list.value[k] - log_norm;
+        const float w = expf(logw);
+        if (list.column[k] >= 0 && w != 0.0f) {
+            const float logq = empty ? -CUDART_INF_F : (student[k] - all.m) * a.inv_t - log_sum;
+            loss += static_cast<double>(w) * (logw - logq);
+        }
+    }
+    loss = warp_sum_f64(loss);
+    if (tid == 0) {
+        if (TAIL && rest > 0.0f) {
+            const float log_rest_q = (rec.m - all.m) * a.inv_t + (tail_log_sum - log_sum);
+            loss += static_cast<double>(rest) * (logf(rest) - log_rest_q);
+        }
+        if (list.bad) atomicOr(a.status, kStatusBadIndex);
+        a.loss[row] = broken ? CUDART_NAN_F : static_cast<float>(loss);
+        float* s = a.stats + row * kStats;
+        s[0] = broken ? CUDART_NAN_F : (no_teacher ? -CUDART_INF_F : all.m);
+        s[1] = log_sum;
+        s[2] = TAIL ? rec.m : all.m;
+        s[3] = TAIL ? tail_log_sum : log_sum;
+        s[4] = log_norm;
+        s[5] = rest;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// backward: elementwise with row scalars; a CTA writes the formula for unlisted columns over its piece of
+// the row and then the listed columns that lie in it
+// ---------------------------------------------------------------------------
+struct DistillBwdArgs {
+    const void* logits;
+    int64_t ld;
+    const int64_t* index;
+    const float* teacher;
+    int top_k;
+    const float* stats;
+    const float* dloss;
+    void* dlogits;
+    int64_t out_ld;
+    int cols;
+    int pieces;
+    float inv_t;
+    int* status;
+};
+
+template <typename T, bool VECTOR>
+__global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(const DistillBwdArgs a) {
+    constexpr int E = Vec<T>::kElems;
+    __shared__ int column[kMaxList];
+    const int64_t row = blockIdx.x / a.pieces;
+    const int piece = static_cast<int>(blockIdx.x % a.pieces);
+    const int tid = threadIdx.x;
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    T* out = static_cast<T*>(a.dlogits) + row * a.out_ld;
+    const float* s = a.stats + row * kStats;
+    const float all_m = s[0], all_log = s[1], tail_m = s[2], tail_log = s[3], log_norm = s[4], rest = s[5];
+    const float k2 = a.inv_t * kLog2e;
+    float g = a.dloss[row] * a.inv_t;
+
+    // this thread's list entry: its column, the student's logit there (before anything is written: the
+    // gradient may take the logits' place) and whether the column lies in this CTA's piece
+    const int64_t given = tid < a.top_k ? a.index[row * a.top_k + tid] : -1;
+    const bool bad = given >= a.cols;
+    const int c = given < 0 || bad ? -1 : static_cast<int>(given);
+    const RowSpan<T> span(x, 0, a.cols);
+    const int v0 = piece * kThreads * kUnroll;   // first vector (or first scalar / E) of the piece
+    auto in_piece = [&](int col) {
+        if (!VECTOR) return col / (kThreads * kUnroll * E) == piece;
+        const int v = col - span.head;
+        if (v < 0 || v >= span.nvec * E) return piece == 0;
+        return v / (kThreads * kUnroll * E) == piece;
+    };
+    const bool mine = c >= 0 && in_piece(c);
+    float xl = 0.0f;
+    if (mine) xl = Vec<T>::load(x + c);
+    if (tid < kMaxList) column[tid] = c;
+    // also the barrier between the loads above and the first write; 1: some column, 2: one outside the row
+    const int seen = (c >= 0 ? 1 : 0) | (bad ? 2 : 0);
+    const int any = (__syncthreads_or(seen & 1) ? 1 : 0) | (__syncthreads_or(seen & 2) ? 2 : 0);
+
+    // no teacher, or no unmasked logit: no gradient
+    const bool zero = any == 0 || all_m == -CUDART_INF_F;
+    if (any & 2) {
+        if (piece == 0 && tid == 0) atomicOr(a.status, kStatusBadIndex);
+        g = CUDART_NAN_F;
+    }
+    if (is_broken(all_m)) g = CUDART_NAN_F;
+    // outside the list: exp(z - tail lse) * (q_r - w_r); tail_m = -inf says that every such logit is masked
+    const float factor = zero ? 0.0f : g * (ex2_approx((tail_m - all_m) * k2 + (tail_log - all_log) * kLog2e) - rest);
+    const float base = tail_m == -CUDART_INF_F ? 0.0f : tail_m, log2_sum = tail_log * kLog2e;
+    auto grad = [&](float xv) { return ex2_approx(fmaf(xv - base, k2, -log2_sum)) * factor; };
+
+    if (!VECTOR) {
+        const int first = v0 * E, last = min(a.cols, first + kThreads * kUnroll * E);
+        for (int i = first + tid; i < last; i += kThreads)
+            Vec<T>::store(out + i, zero ? 0.0f : grad(Vec<T>::load(x + i)));
+    } else {
+        const uint4* in_vec = span.vectors();
+        uint4* out_vec = reinterpret_cast<uint4*>(out + span.head);
+        if (piece == 0 && tid < span.edges) {
+            const int i = span.edge_offset(tid);
+            Vec<T>::store(out + i, zero ? 0.0f : grad(Vec<T>::load(x + i)));
+        }
+        uint4 v[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int i = v0 + tid + u * kThreads;
+            v[u] = !zero && i < span.nvec ? load_stream(in_vec + i) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int i = v0 + tid + u * kThreads;
+            if (i >= span.nvec) break;
+            float y[E];
+            Vec<T>::unpack(v[u], y);
+#pragma unroll
+            for (int j = 0; j < E; ++j) y[j] = zero ? 0.0f : grad(y[j]);
+            __stcs(out_vec + i, Vec<T>::pack(y));
+        }
+    }
+    if (zero) return;
+    __syncthreads();   // the piece is written; the listed columns follow
+    if (mine) {
+        // a column that appears more than once: the first place writes for all, in list order
+        float w = 0.0f;
+        bool earlier = false;
+        for (int k = 0; k < a.top_k; ++k) {
+            if (column[k] == c) {
+                earlier |= k < tid;
+                w += expf(a.teacher[row * a.top_k + k] - log_norm);
+            }
+        }
+        const float q = ex2_approx(fmaf(xl - all_m, k2, -all_log * kLog2e));
+        if (!earlier) Vec<T>::store(out + c, g * (q - w));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+int check_list(const int64_t* index, const float* teacher, int top_k, int64_t rows) {
+    if (top_k < 1 || top_k > kMaxList)
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "top_k must be in [1, %d] (got %d)", kMaxList, top_k);
+    if (rows != 0 && (index == nullptr || teacher == nullptr))
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "teacher_index and teacher_logprob must not be NULL");
+    return CREDIT_OK;
+}
+
+int forward(const void* logits, int64_t ld, const int64_t* index, const float* teacher, int top_k, float* loss,
+            float* stats, int64_t rows, int64_t cols, float temperature, int tail, int dtype,
+            const credit_launch_opts* opts, void* stream) {
+    int rc = check_logits(logits, ld, rows, cols, temperature, dtype);
+    if (rc == CREDIT_OK) rc = check_list(index, teacher, top_k, rows);
+    int cluster = 0;
+    if (rc == CREDIT_OK) rc = check_cluster_only(opts, &cluster);
+    if (rc != CREDIT_OK) return rc;
+    if (rows == 0) return CREDIT_OK;
+    if (loss == nullptr || stats == nullptr)
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "loss and stats must not be NULL");
+    DeviceContext ctx;
+    rc = current_device_context(&ctx);
+    if (rc != CREDIT_OK) return rc;
+    if (cluster == 0) cluster = row_split(rows, cols, ctx.sm_count);
+    DistillArgs a;
+    a.logits = logits;
+    a.ld = ld;
+    a.index = index;
+    a.teacher = teacher;
+    a.top_k = top_k;
+    a.loss = loss;
+    a.stats = stats;
+    a.cols = static_cast<int>(cols);
+    a.slice = row_slice(cols, cluster);
+    if (tail != 0 && a.slice > (1 << 20)) {   // the bitmap of a slice: at most 128 KiB
+        cluster = cluster < 4 ? 4 : cluster;
+        a.slice = row_slice(cols, cluster);
+    }
+    a.bitmap_words = tail != 0 ? (a.slice + 31) / 32 : 0;
+    a.inv_t = 1.0f / temperature;
+    a.status = ctx.status;
+    const void* func;
+    if (dtype == CREDIT_BF16)
+        func = tail ? reinterpret_cast<const void*>(&distill_topk_kernel<__nv_bfloat16, true>)
+                    : reinterpret_cast<const void*>(&distill_topk_kernel<__nv_bfloat16, false>);
+    else
+        func = tail ? reinterpret_cast<const void*>(&distill_topk_kernel<float, true>)
+                    : reinterpret_cast<const void*>(&distill_topk_kernel<float, false>);
+    rc = prepare_kernel(ctx, func);
+    if (rc != CREDIT_OK) return rc;
+    void* args[] = {&a};
+    return launch_kernel(func, rows * cluster, kThreads, cluster, a.bitmap_words * 4, stream, args);
+}
+
+int backward(const void* logits, int64_t ld, const int64_t* index, const float* teacher, int top_k, const float* stats,
+             const float* dloss, void* dlogits, int64_t out_ld, int64_t rows, int64_t cols, float temperature, int dtype,
+             const credit_launch_opts* opts, void* stream) {
+    int rc = check_logits(logits, ld, rows, cols, temperature, dtype);
+    if (rc == CREDIT_OK) rc = check_gradient(logits, ld, dlogits, out_ld, rows, cols, dtype);
+    if (rc == CREDIT_OK) rc = check_list(index, teacher, top_k, rows);
+    int cluster = 0;
+    if (rc == CREDIT_OK) rc = check_cluster_only(opts, &cluster);
+    if (rc != CREDIT_OK) return rc;
+    if (cluster > 1)
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "the gradient is elementwise: cluster_size must be 0 or 1");
+    if (rows == 0) return CREDIT_OK;
+    if (stats == nullptr || dloss == nullptr)
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "stats and dloss must not be NULL");
+    DeviceContext ctx;
+    rc = current_device_context(&ctx);
+    if (rc != CREDIT_OK) return rc;
+    DistillBwdArgs a;
+    a.logits = logits;
+    a.ld = ld;
+    a.index = index;
+    a.teacher = teacher;
+    a.top_k = top_k;
+    a.stats = stats;
+    a.dloss = dloss;
+    a.dlogits = dlogits;
+    a.out_ld = out_ld;
+    a.cols = static_cast<int>(cols);
+    a.inv_t = 1.0f / temperature;
+    a.status = ctx.status;
+    const bool vector = same_phase(logits, ld, dlogits, out_ld, rows, dtype);
+    const int per_piece = kThreads * kUnroll * (dtype == CREDIT_BF16 ? 8 : 4);
+    a.pieces = static_cast<int>((cols + per_piece - 1) / per_piece);
+    const void* func;
+    if (dtype == CREDIT_BF16)
+        func = vector ? reinterpret_cast<const void*>(&distill_topk_bwd_kernel<__nv_bfloat16, true>)
+                      : reinterpret_cast<const void*>(&distill_topk_bwd_kernel<__nv_bfloat16, false>);
+    else
+        func = vector ? reinterpret_cast<const void*>(&distill_topk_bwd_kernel<float, true>)
+                      : reinterpret_cast<const void*>(&distill_topk_bwd_kernel<float, false>);
+    rc = prepare_kernel(ctx, func);
+    if (rc != CREDIT_OK) return rc;
+    void* args[] = {&a};
+    return launch_kernel(func, rows * a.pieces, kThreads, 1, 0, stream, args);
+}
+
+}  // namespace
+}  // namespace credit
+
+extern "C" {
+
+int credit_distill_topk_forward(const void* logits, int64_t row_stride, const int64_t* teacher_index,
+                                const float* teacher_logprob, int top_k, float* loss, float* stats, int64_t rows,
+                                int64_t cols, float temperature, int tail, int dtype, const credit_launch_opts* opts,
+                                void* stream) {
+    return credit::guarded([&] {
+        return credit::forward(logits, row_stride, teacher_index, teacher_logprob, top_k, loss, stats, rows, cols,
+                               temperature, tail, dtype, opts, stream);
+    });
+}
+
+int credit_distill_topk_backward(const void* logits, int64_t row_stride, const int64_t* teacher_index,
+                                 const float* teacher_logprob, int top_k, const float* stats, const float* dloss,
+                                 void* dlogits, int64_t dlogits_row_stride, int64_t rows, int64_t cols, float temperature,
+                                 int dtype, const credit_launch_opts* opts, void* stream) {
+    return credit::guarded([&] {
+        return credit::backward(logits, row_stride, teacher_index, teacher_logprob, top_k, stats, dloss, dlogits,
+                                dlogits_row_stride, rows, cols, temperature, dtype, opts, stream);
+    });
+}
+
+}  // extern "C"

@@ -20,6 +20,7 @@
 
 #include "../../include/credit_b200.h"
 #include "cluster_primitives.cuh"
+#include "device_context.h"
 #include "error_state.h"
 #include "kernel_tables.h"
 #include "launch_args.h"
@@ -847,6 +848,55 @@ StagedArgs staged_args(const Resolved& r) {
 }
 
 }  // namespace
+
+int current_device_context(DeviceContext* out) {
+    DeviceState* st = nullptr;
+    CREDIT_CUDA_TRY(cudaGetDevice(&out->device));
+    int rc = load_device(out->device, &st);
+    if (rc != CREDIT_OK) return rc;
+    out->sm_count = st->info.sm_count;
+    out->max_dynamic_smem = st->info.max_dynamic_smem_per_block;
+    out->status = st->status_ptr;
+    return CREDIT_OK;
+}
+
+int prepare_kernel(const DeviceContext& ctx, const void* func) {
+    return prepare_function(ctx.device, func, ctx.max_dynamic_smem);
+}
+
+int resident_clusters(const DeviceContext& ctx, const void* func, int cluster, int smem, int threads, int* out) {
+    return max_active_clusters(ctx.device, func, cluster, smem, threads, out);
+}
+
+int launch_kernel(const void* func, int64_t grid, int threads, int cluster, int smem, void* stream, void** args) {
+    if (grid > 0x7fffffffll)
+        return fail(CREDIT_ERR_UNSUPPORTED, "the call needs %lld thread blocks, more than one launch takes",
+                    static_cast<long long>(grid));
+    Launch l;
+    l.func = func;
+    l.grid = static_cast<int>(grid);
+    l.threads = threads;
+    l.cluster = cluster;
+    l.smem = smem;
+    l.stream = static_cast<cudaStream_t>(stream);
+    return launch_cluster_kernel(l, args);
+}
+
+int check_matrix_shape(int64_t rows, int64_t cols, int dtype) {
+    Shape s;
+    return check_shape(rows, cols, dtype, &s);
+}
+
+int check_cluster_only(const credit_launch_opts* opts, int* cluster) {
+    credit_launch_opts o;
+    int rc = check_opts(opts, &o);
+    if (rc != CREDIT_OK) return rc;
+    if (o.variant || o.stages || o.threads || o.schedule || o.load_path || o.chunk_bytes || o.flags)
+        return fail(CREDIT_ERR_INVALID_ARGUMENT, "of the launch options this call takes cluster_size only");
+    *cluster = o.cluster_size;
+    return CREDIT_OK;
+}
+
 }  // namespace credit
 
 using namespace credit;
@@ -875,7 +925,7 @@ int credit_device_status(int* status_out, int reset) {
     if (reset && word != 0) CREDIT_CUDA_TRY(cudaMemset(st->status_ptr, 0, sizeof(int)));
     if (status_out != nullptr) *status_out = word;
     if (word != 0)
-        return fail(CREDIT_ERR_DEVICE_STATUS, "device status word = %d (1: wait timed out, 2: bad geometry)",
+        return fail(CREDIT_ERR_DEVICE_STATUS, "device status word = %d (1: wait timed out, 2: bad geometry, 4: column index out of range)",
                     word);
     return CREDIT_OK;
 }

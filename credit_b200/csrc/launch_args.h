@@ -21,6 +21,7 @@ constexpr int kControlBytes = 4096;
 // Bits of the device status word (see credit_device_status in the C ABI).
 constexpr int kStatusWaitTimeout = 1;      // an mbarrier wait ran out of patience
 constexpr int kStatusBadGeometry = 2;      // a kernel saw a launch shape it cannot handle
+constexpr int kStatusBadIndex = 4;         // a given column index lies outside the row
 
 // Geometry shared by the staged kernels.
 struct StagedArgs {

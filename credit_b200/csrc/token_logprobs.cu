@@ -1,0 +1,416 @@
+// Log probabilities of given tokens with the row's entropy and top alternatives, and the gradient of
+// the first two with respect to the logits. With z = x / temperature over a row of `cols` logits:
+//   S = sum_j exp(z_j - z_max),  logprob = z_t - z_max - log S,  H = log S - sum_j p_j (z_j - z_max),
+//   dlogits_j = (g (delta_jt - p_j) - gH p_j (log p_j + H)) / temperature.
+// No reference kernel exists for these; the cluster split and the exchange of partial records through
+// distributed shared memory are those of the softmax backward family
+// (src/workloads/softmax_logits_backward.cu:410).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+
+#include "device_context.h"
+#include "top_keys.cuh"
+#include "vocab_host.h"
+
+namespace credit {
+namespace {
+
+constexpr int kThreads = kTopThreads;
+constexpr int kUnroll = 4;
+
+struct LogprobArgs {
+    const void* logits;
+    int64_t ld;
+    const int64_t* targets;   // NULL: no token asked for
+    float* logprob;
+    float* stats;             // [rows, 2]
+    float* entropy;
+    float* top_logprob;       // [rows, top_k]
+    int64_t* top_index;
+    int top_k;
+    int cols;
+    int slice;                // columns per CTA of the cluster
+    float inv_t;
+    int* status;
+};
+
+// ---------------------------------------------------------------------------
+// forward: one cluster per row, the row read once
+// ---------------------------------------------------------------------------
+template <typename T, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobArgs a) {
+    __shared__ SoftmaxRecord warp_records[kThreads / 32];
+    __shared__ SoftmaxRecord records[kMaxClusterSize];   // rank 0: one per CTA
+    __shared__ float row_max, row_log_sum;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    TopBuffer& t = *reinterpret_cast<TopBuffer*>(dynamic);
+
+    const uint32_t rank = cluster_cta_rank(), nranks = cluster_cta_count();
+    const int64_t row = blockIdx.x / nranks;
+    const int tid = threadIdx.x;
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+
+    int64_t target = 0;
+    if (a.targets != nullptr) {
+        target = a.targets[row];
+        if (target < 0) {   // ignored row: nothing is read (the whole cluster leaves here)
+            if (rank == 0) {
+                if (tid == 0) {
+                    a.logprob[row] = 0.0f;
+                    a.stats[2 * row] = a.stats[2 * row + 1] = 0.0f;
+                    if (ENTROPY) a.entropy[row] = 0.0f;
+                }
+                if (TOP && tid < a.top_k) {
+                    a.top_logprob[row * a.top_k + tid] = -CUDART_INF_F;
+                    a.top_index[row * a.top_k + tid] = -1;
+                }
+            }
+            return;
+        }
+    }
+    if (!TOP) cluster_arrive_release();   // "this CTA runs": its shared memory may be written from now on
+    float picked = CUDART_NAN_F;
+    if (a.targets != nullptr && rank == 0 && tid == 0) {
+        if (target < a.cols) {
+            picked = Vec<T>::load(x + target);
+        } else {
+            atomicOr(a.status, kStatusBadIndex);
+        }
+    }
+    if (TOP && tid == 0) init_top_buffer(t);
+
+    const int start = static_cast<int>(rank) * a.slice;
+    const int local = max(0, min(a.slice, a.cols - start));
+    const RowSpan<T> span(x, start, local);
+    const float k2 = a.inv_t * kLog2e;
+    SoftmaxRecord rec = empty_record();
+    TopCollector<T> collector(t, a.top_k);
+    int next_tighten = 4;
+    constexpr int kStride = kThreads * Vec<T>::kElems;
+    stream_slice<T, kThreads, kUnroll>(
+        span,
+        [&](const uint4 (&v)[kUnroll], int first, int it) {
+            float part[kUnroll];
+            const float top = chunk_max<T>(v, part);
+            if (TOP) {
+                const int column = span.vector_column(first);
+                if (it == 0) {
+                    collector.first_threshold(v, part, top, column, kStride);
+                } else if (it == next_tighten) {
+                    collector.tighten();
+                    next_tighten *= 4;
+                }
+                collector.offer_chunk(v, part, top, column, kStride);
+            }
+            accumulate<T, kUnroll, ENTROPY>(v, top, k2, rec);
+        },
+        [&](const uint4 (&v)[1]) {
+            const float top = Vec<T>::max(v[0]);
+            if (TOP) {
+                if (span.nvec == 0) __syncthreads();   // the buffer's first use
+                if (tid < span.edges) {
+                    float e[Vec<T>::kElems];
+                    Vec<T>::unpack(v[0], e);
+                    collector.offer(e[0], span.start + span.edge_offset(tid));
+                }
+            }
+            accumulate<T, 1, ENTROPY>(v, top, k2, rec);
+        });
+
+    rec = cta_record<kThreads>(rec, warp_records, k2);
+    if (TOP) collector.finish(span);
+    if (nranks > 1) {
+        if (TOP) cluster_arrive_release();   // this CTA's list is ready and its buffer may be written
+        cluster_wait_acquire();
+        if (rank != 0) {
+            if (tid == 0) {
+                const uint32_t to = map_to_rank(smem_u32(&records[rank]), 0);
+                st_cluster_f32(to, rec.m);
+                st_cluster_f32(to + 4, rec.s);
+                st_cluster_f32(to + 8, rec.e);
+            }
+            if (TOP && tid < a.top_k)
+                st_cluster_u64(map_to_rank(smem_u32(&t.keys[rank * a.top_k + tid]), 0), tid < t.fill ? t.keys[tid] : 0);
+        } else if (TOP && tid < a.top_k && tid >= t.fill) {
+            t.keys[tid] = 0;
+        }
+        cluster_sync_all();
+        if (rank != 0) return;
+        if (TOP) keep_largest(t, static_cast<int>(nranks) * a.top_k, a.top_k);
+    } else if (!TOP) {
+        cluster_wait_acquire();
+    }
+
+    if (tid == 0) {
+        for (uint32_t r = 1; r < nranks; ++r) rec = merge_records(rec, records[r], k2);
+        const bool broken = is_broken(rec.m), empty = rec.m == -CUDART_INF_F;
+        const float log_sum = broken ? CUDART_NAN_F : (empty ? 0.0f : logf(rec.s));
+        row_max = rec.m;
+        row_log_sum = log_sum;
+        a.stats[2 * row] = rec.m;
+        a.stats[2 * row + 1] = log_sum;
+        if (a.targets != nullptr)
+            a.logprob[row] = empty && target < a.cols ? -CUDART_INF_F : (picked - rec.m) * a.inv_t - log_sum;
+        if (ENTROPY) a.entropy[row] = broken ? CUDART_NAN_F : (empty ? 0.0f : log_sum - kLn2 * (rec.e / rec.s));
+    }
+    if (TOP) {
+        __syncthreads();
+        const int n = min(t.fill, a.top_k);
+        if (tid < a.top_k) {
+            const int64_t base = row * a.top_k;
+            if (tid < n) {
+                const uint64_t key = t.keys[tid];
+                int place = 0;
+                for (int i = 0; i < n; ++i) place += t.keys[i] > key;
+                a.top_logprob[base + place] = (key_value(key) - row_max) * a.inv_t - row_log_sum;
+                a.top_index[base + place] = key_column(key);
+            } else {
+                a.top_logprob[base + tid] = -CUDART_INF_F;
+                a.top_index[base + tid] = -1;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// backward: elementwise with row scalars, the logits read once and the gradient written once
+// ---------------------------------------------------------------------------
+struct LogprobBwdArgs {
+    const void* logits;
+    int64_t ld;
+    const int64_t* targets;
+    const float* stats;
+    const float* entropy;    // with dentropy
+    const float* dlogprob;
+    const float* dentropy;   // NULL: none
+    void* dlogits;
+    int64_t out_ld;
+    int cols;
+    int pieces;              // CTAs per row
+    float inv_t;
+    int* status;
+};
+
+struct LogprobRow {
+    float base, k2, log2_sum;   // log2 p = (x - base) * k2 - log2_sum
+    float g, gh, h2;            // upstream gradients over the temperature, entropy / ln 2
+    int target;
+};
+
+template <bool ENTROPY>
+__device__ __forceinline__ float logprob_grad(float x, const LogprobRow& r) {
+    float d = fmaf(x - r.base, r.k2, -r.log2_sum);
+    if (ENTROPY) {
+        d = fmaxf(d, -200.0f);   // p = 0 there, and 0 * -inf is kept out
+        return -ex2_approx(d) * fmaf(r.gh, d + r.h2, r.g);
+    }
+    return -ex2_approx(d) * r.g;
+}
+
+template <typename T, bool ENTROPY, bool VECTOR>
+__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const LogprobBwdArgs a) {
+    const int64_t row = blockIdx.x / a.pieces;
+    const int piece = static_cast<int>(blockIdx.x % a.pieces);
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    T* out = static_cast<T*>(a.dlogits) + row * a.out_ld;
+    const int64_t target = a.targets[row];
+    LogprobRow r;
+    r.base = a.stats[2 * row];
+    r.k2 = a.inv_t * kLog2e;
+    r.log2_sum = a.stats[2 * row + 1] * kLog2e;
+    r.g = a.dlogprob[row] * a.inv_t;
+    r.gh = ENTROPY ? a.dentropy[row] * a.inv_t * kLn2 : 0.0f;
+    r.h2 = ENTROPY ? a.entropy[row] * kLog2e : 0.0f;
+    r.target = static_cast<int>(target);
+    // an ignored row, or one without an unmasked logit: no gradient
+    const bool zero = target < 0 || r.base == -CUDART_INF_F;
+    if (target >= a.cols) {
+        if (piece == 0 && threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
+        r.g = CUDART_NAN_F;
+    }
+    if (is_broken(r.base)) r.g = CUDART_NAN_F;   // NaN or +inf in the row: NaN throughout
+    // at the target: + g, with 1 - p taken by expm1 so that nothing cancels when p is near 1
+    auto at_target = [&](float xv) {
+        const float d = fmaf(xv - r.base, r.k2, -r.log2_sum);
+        const float dc = fmaxf(d, -200.0f);
+        const float entropy_part = ENTROPY ? -ex2_approx(dc) * r.gh * (dc + r.h2) : 0.0f;
+        return fmaf(r.g, -expm1f(d * kLn2), entropy_part);
+    };
+    auto grad = [&](float xv, int column) {
+        if (zero) return 0.0f;
+        return column == r.target ? at_target(xv) : logprob_grad<ENTROPY>(xv, r);
+    };
+
+    if (!VECTOR) {
+        const int first = piece * kThreads * kUnroll * Vec<T>::kElems;
+        const int last = min(a.cols, first + kThreads * kUnroll * Vec<T>::kElems);
+        for (int c = first + static_cast<int>(threadIdx.x); c < last; c += kThreads)
+            Vec<T>::store(out + c, grad(zero ? 0.0f : Vec<T>::load(x + c), c));
+        return;
+    }
+    constexpr int E = Vec<T>::kElems;
+    const RowSpan<T> span(x, 0, a.cols);
+    const uint4* in_vec = span.vectors();
+    uint4* out_vec = reinterpret_cast<uint4*>(out + span.head);
+    if (piece == 0 && static_cast<int>(threadIdx.x) < span.edges) {
+        const int c = span.edge_offset(threadIdx.x);
+        Vec<T>::store(out + c, grad(zero ? 0.0f : Vec<T>::load(x + c), c));
+    }
+    const int i0 = piece * kThreads * kUnroll + static_cast<int>(threadIdx.x);
+    uint4 v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+        v[u] = !zero && i0 + u * kThreads < span.nvec ? load_stream(in_vec + i0 + u * kThreads) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const int i = i0 + u * kThreads;
+        if (i >= span.nvec) break;
+        float y[E];
+        if (zero) {
+            __stcs(out_vec + i, make_uint4(0, 0, 0, 0));
+            continue;
+        }
+        Vec<T>::unpack(v[u], y);
+        const int hit = r.target - span.vector_column(i);
+        const float picked = hit >= 0 && hit < E ? at_target(Vec<T>::load(x + r.target)) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) y[j] = j == hit ? picked : logprob_grad<ENTROPY>(y[j], r);
+        __stcs(out_vec + i, Vec<T>::pack(y));
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+template <typename T>
+const void* forward_kernel(bool entropy, bool top) {
+    if (entropy)
+        return top ? reinterpret_cast<const void*>(&token_logprobs_kernel<T, true, true>)
+                   : reinterpret_cast<const void*>(&token_logprobs_kernel<T, true, false>);
+    return top ? reinterpret_cast<const void*>(&token_logprobs_kernel<T, false, true>)
+               : reinterpret_cast<const void*>(&token_logprobs_kernel<T, false, false>);
+}
+
+template <typename T>
+const void* backward_kernel(bool entropy, bool vector) {
+    if (entropy)
+        return vector ? reinterpret_cast<const void*>(&token_logprobs_bwd_kernel<T, true, true>)
+                      : reinterpret_cast<const void*>(&token_logprobs_bwd_kernel<T, true, false>);
+    return vector ? reinterpret_cast<const void*>(&token_logprobs_bwd_kernel<T, false, true>)
+                  : reinterpret_cast<const void*>(&token_logprobs_bwd_kernel<T, false, false>);
+}
+
+int forward(const void* logits, int64_t ld, const int64_t* targets, float* logprob, float* stats, float* entropy,
+            float* top_logprob, int64_t* top_index, int top_k, int64_t rows, int64_t cols, float temperature, int dtype,
+            const credit_launch_opts* opts, void* stream) {
+    int rc = check_logits(logits, ld, rows, cols, temperature, dtype);
+    if (rc != CREDIT_OK) return rc;
+    int cluster = 0;
+    rc = check_cluster_only(opts, &cluster);
+    if (rc != CREDIT_OK) return rc;
+    if (top_k < 0 || top_k > kMaxTop)
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "top_k must be in [0, %d] (got %d)", kMaxTop, top_k);
+    if (rows == 0) return CREDIT_OK;
+    if (stats == nullptr || (targets == nullptr) != (logprob == nullptr))
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "stats must not be NULL, targets and logprob go together");
+    if (targets == nullptr && top_k == 0 && entropy == nullptr)
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "nothing is asked for: targets, entropy and top_k are all absent");
+    if (top_k > 0 && (top_logprob == nullptr || top_index == nullptr))
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "top_k = %d needs top_logprob and top_index", top_k);
+    DeviceContext ctx;
+    rc = current_device_context(&ctx);
+    if (rc != CREDIT_OK) return rc;
+    if (cluster == 0) cluster = row_split(rows, cols, ctx.sm_count);
+    LogprobArgs a;
+    a.logits = logits;
+    a.ld = ld;
+    a.targets = targets;
+    a.logprob = logprob;
+    a.stats = stats;
+    a.entropy = entropy;
+    a.top_logprob = top_logprob;
+    a.top_index = top_index;
+    a.top_k = top_k;
+    a.cols = static_cast<int>(cols);
+    a.slice = row_slice(cols, cluster);
+    a.inv_t = 1.0f / temperature;
+    a.status = ctx.status;
+    const bool top = top_k > 0;
+    const void* func = dtype == CREDIT_BF16 ? forward_kernel<__nv_bfloat16>(entropy != nullptr, top)
+                                            : forward_kernel<float>(entropy != nullptr, top);
+    rc = prepare_kernel(ctx, func);
+    if (rc != CREDIT_OK) return rc;
+    void* args[] = {&a};
+    return launch_kernel(func, rows * cluster, kThreads, cluster, top ? static_cast<int>(sizeof(TopBuffer)) : 0, stream, args);
+}
+
+int backward(const void* logits, int64_t ld, const int64_t* targets, const float* stats, const float* entropy,
+             const float* dlogprob, const float* dentropy, void* dlogits, int64_t out_ld, int64_t rows, int64_t cols,
+             float temperature, int dtype, const credit_launch_opts* opts, void* stream) {
+    int rc = check_logits(logits, ld, rows, cols, temperature, dtype);
+    if (rc == CREDIT_OK) rc = check_gradient(logits, ld, dlogits, out_ld, rows, cols, dtype);
+    int cluster = 0;
+    if (rc == CREDIT_OK) rc = check_cluster_only(opts, &cluster);
+    if (rc != CREDIT_OK) return rc;
+    if (cluster > 1)
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "the gradient is elementwise: cluster_size must be 0 or 1");
+    if (rows == 0) return CREDIT_OK;
+    if (targets == nullptr || stats == nullptr || dlogprob == nullptr)
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "targets, stats and dlogprob must not be NULL");
+    if (dentropy != nullptr && entropy == nullptr)
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "dentropy needs the entropy of the forward pass");
+    DeviceContext ctx;
+    rc = current_device_context(&ctx);
+    if (rc != CREDIT_OK) return rc;
+    LogprobBwdArgs a;
+    a.logits = logits;
+    a.ld = ld;
+    a.targets = targets;
+    a.stats = stats;
+    a.entropy = entropy;
+    a.dlogprob = dlogprob;
+    a.dentropy = dentropy;
+    a.dlogits = dlogits;
+    a.out_ld = out_ld;
+    a.cols = static_cast<int>(cols);
+    a.inv_t = 1.0f / temperature;
+    a.status = ctx.status;
+    const bool vector = same_phase(logits, ld, dlogits, out_ld, rows, dtype);
+    const int per_piece = kThreads * kUnroll * (dtype == CREDIT_BF16 ? 8 : 4);
+    a.pieces = static_cast<int>((cols + per_piece - 1) / per_piece);
+    const void* func = dtype == CREDIT_BF16 ? backward_kernel<__nv_bfloat16>(dentropy != nullptr, vector)
+                                            : backward_kernel<float>(dentropy != nullptr, vector);
+    rc = prepare_kernel(ctx, func);
+    if (rc != CREDIT_OK) return rc;
+    void* args[] = {&a};
+    return launch_kernel(func, rows * a.pieces, kThreads, 1, 0, stream, args);
+}
+
+}  // namespace
+}  // namespace credit
+
+extern "C" {
+
+int credit_token_logprobs_forward(const void* logits, int64_t row_stride, const int64_t* targets, float* logprob,
+                                  float* stats, float* entropy, float* top_logprob, int64_t* top_index, int top_k,
+                                  int64_t rows, int64_t cols, float temperature, int dtype, const credit_launch_opts* opts,
+                                  void* stream) {
+    return credit::guarded([&] {
+        return credit::forward(logits, row_stride, targets, logprob, stats, entropy, top_logprob, top_index, top_k, rows,
+                               cols, temperature, dtype, opts, stream);
+    });
+}
+
+int credit_token_logprobs_backward(const void* logits, int64_t row_stride, const int64_t* targets, const float* stats,
+                                   const float* entropy, const float* dlogprob, const float* dentropy, void* dlogits,
+                                   int64_t dlogits_row_stride, int64_t rows, int64_t cols, float temperature, int dtype,
+                                   const credit_launch_opts* opts, void* stream) {
+    return credit::guarded([&] {
+        return credit::backward(logits, row_stride, targets, stats, entropy, dlogprob, dentropy, dlogits,
+                                dlogits_row_stride, rows, cols, temperature, dtype, opts, stream);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,295 @@
+// The k largest of a row slice that is read once: candidates collect in a shared-memory buffer, a
+// threshold (always the key of a real element that k elements reach) keeps the rest out.
+//
+// Order. An element is the 64-bit key (monotone image of its value, complement of its column): larger
+// keys first is "value descending, column ascending", all keys of a row differ, so the chosen set
+// does not depend on the order in which threads append. NaN ranks above +inf, -0 equals +0, -inf is
+// never an element (its image lies under kLowestKey).
+//
+// The threshold starts at the k-th largest of the threads' first-chunk maxima and is tightened after
+// chunks 4, 16, 64, ...: on rows in no particular order each interval then adds about 3k candidates,
+// so 2048 places hold every k up to 128. A row that brings more (sorted ascending, say) overflows; its
+// slice is then searched by the digit-by-digit selection straight from global memory, at most 8 more
+// reads of it.
+#pragma once
+
+#include "vocab_rows.cuh"
+
+namespace credit {
+
+constexpr int kMaxTop = 128;
+constexpr int kTopThreads = 256;
+constexpr int kTopCapacity = 2048;   // kMaxClusterSize * kMaxTop: rank 0 gathers every CTA's list in it
+static_assert(kTopCapacity >= kMaxClusterSize * kMaxTop, "the gathered lists must fit");
+constexpr uint64_t kLowestKey = 0x0080000000000000ull;   // the image of -FLT_MAX, any column
+
+__device__ __forceinline__ uint32_t ordered_image(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);   // -0 + 0 = +0
+    if (x != x) return 0xffffffffu;
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+__device__ __forceinline__ float image_value(uint32_t k) {
+    return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
+}
+
+__device__ __forceinline__ uint64_t element_key(float x, int column) {
+    return (static_cast<uint64_t>(ordered_image(x)) << 32) | (0xffffffffu - static_cast<uint32_t>(column));
+}
+
+__device__ __forceinline__ float key_value(uint64_t key) { return image_value(static_cast<uint32_t>(key >> 32)); }
+__device__ __forceinline__ int key_column(uint64_t key) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key)); }
+
+struct TopBuffer {
+    unsigned long long keys[kTopCapacity];
+    unsigned int hist[256];
+    unsigned long long lowest;   // smallest kept key
+    unsigned int differ[2];      // bits in which the keys differ (high, low word); zero between calls
+    int count;                   // candidates appended (may exceed the capacity)
+    int fill, digit, above, here;
+};
+
+// By one thread, before the first barrier.
+__device__ __forceinline__ void init_top_buffer(TopBuffer& t) {
+    t.count = 0;
+    t.differ[0] = t.differ[1] = 0;
+}
+
+// Warp 0: the digit in which the need-th largest lies, how many lie above it and in it.
+__device__ __forceinline__ void find_digit(TopBuffer& t, int need) {
+    const int lane = threadIdx.x & 31;
+    int part[8], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        part[j] = static_cast<int>(t.hist[255 - 8 * lane - j]);
+        sum += part[j];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    int before = upto - sum;
+    if (before < need && upto >= need) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (before < need && before + part[j] >= need) {
+                t.digit = 255 - 8 * lane - j;
+                t.above = before;
+                t.here = part[j];
+            }
+            before += part[j];
+        }
+    }
+}
+
+// Keeps the k largest of keys[0, n), n <= kTopCapacity (fewer when fewer are non-zero: zeros are
+// empty places), and returns the smallest of them (0 when there are fewer than k). All threads call
+// it behind a barrier; it ends with one, the number kept in t.fill.
+__device__ __forceinline__ uint64_t keep_largest(TopBuffer& t, int n, int k) {
+    constexpr int kPer = kTopCapacity / kTopThreads;
+    const int tid = threadIdx.x;
+    uint64_t mine[kPer];
+    const uint64_t some = t.keys[0];
+    uint64_t diff = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int i = tid + j * kTopThreads;
+        mine[j] = i < n ? t.keys[i] : some;
+        diff |= mine[j] ^ some;
+        if (i >= n) mine[j] = 0;
+    }
+    const uint32_t hi = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(diff >> 32));
+    const uint32_t lo = __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(diff));
+    if ((tid & 31) == 0) {
+        if (hi != 0) atomicOr(&t.differ[0], hi);
+        if (lo != 0) atomicOr(&t.differ[1], lo);
+    }
+    __syncthreads();
+    diff = (static_cast<uint64_t>(t.differ[0]) << 32) | t.differ[1];
+    uint64_t threshold = some;
+    if (diff != 0 && n > k) {
+        int bits = 64 - __clzll(static_cast<long long>(diff));   // undecided low bits
+        uint64_t mask = bits == 64 ? 0 : ~0ull << bits;
+        threshold = some & mask;
+        int need = k;
+        while (bits > 0) {
+            const int shift = bits > 8 ? bits - 8 : 0;
+            const uint32_t digits = (1u << (bits - shift)) - 1u;
+            t.hist[tid] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                if (tid + j * kTopThreads < n && ((mine[j] ^ threshold) & mask) == 0)
+                    atomicAdd(&t.hist[static_cast<uint32_t>(mine[j] >> shift) & digits], 1u);
+            __syncthreads();
+            if (tid < 32) find_digit(t, need);
+            __syncthreads();
+            threshold |= static_cast<uint64_t>(t.digit) << shift;
+            mask |= static_cast<uint64_t>(digits) << shift;
+            need -= t.above;
+            bits = shift;
+            if (t.here == need) break;
+        }
+    } else if (n <= k) {
+        threshold = 0;
+    }
+    if (tid == 0) {
+        t.fill = 0;
+        t.lowest = ~0ull;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        if (mine[j] != 0 && mine[j] >= threshold) {
+            t.keys[atomicAdd(&t.fill, 1)] = mine[j];
+            atomicMin(&t.lowest, static_cast<unsigned long long>(mine[j]));
+        }
+    }
+    if (tid == 0) t.differ[0] = t.differ[1] = 0;
+    __syncthreads();
+    return t.fill < k ? 0 : t.lowest;
+}
+
+// The slow path: the same selection straight from the slice in global memory. Leaves at most k keys
+// in keys[0, fill) and ends with a barrier.
+template <typename T>
+__device__ __noinline__ void select_from_slice(const T* first, int start, int local, int k, TopBuffer& t) {
+    const int tid = threadIdx.x;
+    uint64_t threshold = 0, mask = 0;
+    int need = k;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        t.hist[tid] = 0;
+        if (tid == 0) t.digit = -1;
+        __syncthreads();
+        for (int base = 0; base < local; base += kTopThreads) {
+            int digit = -1;
+            if (base + tid < local) {
+                const uint64_t key = element_key(Vec<T>::load(first + base + tid), start + base + tid);
+                if (key >= kLowestKey && ((key ^ threshold) & mask) == 0) digit = static_cast<int>(key >> shift) & 255;
+            }
+            int same;   // rows of one value: one addition a warp
+            __match_all_sync(0xffffffffu, digit, &same);
+            if (same) {
+                if (digit >= 0 && (tid & 31) == 0) atomicAdd(&t.hist[digit], 32u);
+            } else if (digit >= 0) {
+                atomicAdd(&t.hist[digit], 1u);
+            }
+        }
+        __syncthreads();
+        if (tid < 32) find_digit(t, need);
+        __syncthreads();
+        const int digit = t.digit;
+        if (digit < 0) break;   // (first digit only) fewer than k elements: all of them
+        threshold |= static_cast<uint64_t>(digit) << shift;
+        mask |= 255ull << shift;
+        need -= t.above;
+        const int here = t.here;
+        __syncthreads();
+        if (here == need) break;
+    }
+    if (threshold < kLowestKey) threshold = kLowestKey;
+    if (tid == 0) t.fill = 0;
+    __syncthreads();
+    for (int c = tid; c < local; c += kTopThreads) {
+        const uint64_t key = element_key(Vec<T>::load(first + c), start + c);
+        if (key >= threshold) {
+            const int at = atomicAdd(&t.fill, 1);
+            if (at < kTopCapacity) t.keys[at] = key;
+        }
+    }
+    __syncthreads();
+}
+
+// One CTA's candidates while its slice streams by.
+template <typename T>
+struct TopCollector {
+    TopBuffer& t;
+    const int k;
+    uint64_t key;    // threshold
+    float value;     // its value (+inf when that is NaN, which then lets NaN and +inf through)
+    bool overflow;
+
+    __device__ __forceinline__ TopCollector(TopBuffer& t_, int k_) : t(t_), k(k_), key(kLowestKey), overflow(false) {
+        set_threshold(kLowestKey);
+    }
+
+    __device__ __forceinline__ void set_threshold(uint64_t to) {
+        if (to > key) key = to;
+        value = key_value(key);
+        if (value != value) value = CUDART_INF_F;
+    }
+
+    // The first chunk: every thread's largest element competes.
+    template <int U>
+    __device__ __forceinline__ void first_threshold(const uint4 (&v)[U], const float (&part)[U], float top, int column,
+                                                    int stride) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int u = U - 1; u >= 0; --u) {
+            if (part[u] == top || part[u] != part[u]) {   // columns descend: the lowest one stays
+                float x[Vec<T>::kElems];
+                Vec<T>::unpack(v[u], x);
+#pragma unroll
+                for (int j = Vec<T>::kElems - 1; j >= 0; --j)
+                    if (x[j] == top || x[j] != x[j]) best = element_key(x[j], column + u * stride + j);
+            }
+        }
+        t.keys[threadIdx.x] = best >= kLowestKey ? best : 0;
+        __syncthreads();
+        set_threshold(keep_largest(t, kTopThreads, k));
+        __syncthreads();   // the places are free again before anyone appends
+    }
+
+    // Between chunks: keep the k largest so far.
+    __device__ __forceinline__ void tighten() {
+        __syncthreads();
+        const int n = t.count;
+        __syncthreads();   // everyone has read it before anyone appends again
+        if (n > kTopCapacity) overflow = true;
+        if (n > k && !overflow) {
+            set_threshold(keep_largest(t, n, k));
+            if (threadIdx.x == 0) t.count = t.fill;
+            __syncthreads();
+        }
+    }
+
+    __device__ __forceinline__ void offer(float x, int column) {
+        if (x < value) return;
+        const uint64_t c = element_key(x, column);
+        if (c < key) return;
+        const int at = atomicAdd(&t.count, 1);
+        if (at < kTopCapacity) t.keys[at] = c;
+    }
+
+    template <int U>
+    __device__ __forceinline__ void offer_chunk(const uint4 (&v)[U], const float (&part)[U], float top, int column,
+                                                int stride) {
+        if (top < value || overflow) return;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (part[u] < value) continue;
+            float x[Vec<T>::kElems];
+            Vec<T>::unpack(v[u], x);
+#pragma unroll
+            for (int j = 0; j < Vec<T>::kElems; ++j) offer(x[j], column + u * stride + j);
+        }
+    }
+
+    // The k largest of the slice in keys[0, fill), behind a barrier.
+    __device__ __forceinline__ void finish(const RowSpan<T>& span) {
+        __syncthreads();
+        const int n = t.count;
+        if (n > kTopCapacity || overflow) {
+            select_from_slice(span.first, span.start, span.local, k, t);
+        } else if (n > k) {
+            keep_largest(t, n, k);
+        } else {
+            if (threadIdx.x == 0) t.fill = n;
+            __syncthreads();
+        }
+    }
+};
+
+}  // namespace credit

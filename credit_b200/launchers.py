@@ -204,6 +204,224 @@ def launch_ffn_forward(inputs, outputs, cluster_size: int = 0, opts=None, eps: f
             workspace.data_ptr(), workspace.numel(), _stream_ptr()))
 
 
+def _check_like(name: str, t, x: torch.Tensor, dtype, shape) -> None:
+    """A tensor that must lie beside `x`: the checks of `_check_matrix` and the same device."""
+    _check_matrix(name, t, dtype, shape)
+    if t.device != x.device:
+        raise ValueError(f"{name} must be on {x.device}, got {t.device}")
+
+
+def _ptr(t) -> "int | None":
+    """Device address, or NULL for an absent or empty tensor."""
+    return None if t is None or t.numel() == 0 else t.data_ptr()
+
+
+def launch_residual_norm_forward(inputs, outputs, cluster_size: int = 0, opts=None, residual_scale: float = 1.0,
+                                 eps: float = 1.0e-6) -> None:
+    """The norms after and before a block with its gate and the scaled residual:
+
+        n = rmsnorm(block) * post_weight   (block without post_weight)
+        residual_out = residual_scale * residual + gate * n;   y = rmsnorm(residual_out) * pre_weight
+
+    inputs = (block, residual, post_weight | None, gate | None, pre_weight), outputs = (residual_out, y,
+    post_rstd | None, pre_rstd). residual_out may be residual or block, y block or residual."""
+    block, residual, post_weight, gate, pre_weight = inputs
+    residual_out, y, post_rstd, pre_rstd = outputs
+    _check_matrix("block", block)
+    rows, cols = block.shape
+    for name, t in (("residual", residual), ("residual_out", residual_out), ("y", y)):
+        _check_like(name, t, block, block.dtype, (rows, cols))
+    for name, t in (("post_weight", post_weight), ("gate", gate), ("pre_weight", pre_weight)):
+        if t is not None or name == "pre_weight":
+            _check_like(name, t, block, torch.float32, (cols,))
+    if (post_weight is None) != (post_rstd is None):
+        raise ValueError("post_weight and post_rstd go together")
+    for name, t in (("post_rstd", post_rstd), ("pre_rstd", pre_rstd)):
+        if t is not None or name == "pre_rstd":
+            _check_like(name, t, block, torch.float32, (rows,))
+    o = _opts(cluster_size, opts)
+    with torch.cuda.device(block.device):
+        N.check(N.load().credit_residual_norm_forward(
+            _ptr(block), _ptr(residual), _ptr(post_weight), _ptr(gate), _ptr(pre_weight), _ptr(residual_out), _ptr(y),
+            _ptr(post_rstd), _ptr(pre_rstd), rows, cols, residual_scale, eps, _row_dtype(block), _ref(o), _stream_ptr()))
+
+
+def residual_norm_backward_workspace_bytes(rows: int, cols: int, dtype: torch.dtype, cluster_size: int = 0,
+                                           opts=None) -> int:
+    """For the current device; enough for every call of the shape, with or without post norm."""
+    return int(N.load().credit_residual_norm_backward_workspace_bytes(
+        rows, cols, _DTYPES[dtype], _ref(_opts(cluster_size, opts))))
+
+
+def launch_residual_norm_backward(inputs, outputs, cluster_size: int = 0, opts=None, residual_scale: float = 1.0,
+                                  workspace: torch.Tensor | None = None) -> None:
+    """Gradient of `launch_residual_norm_forward`. inputs = (dy, dresidual_out | None, block, residual_out,
+    post_weight | None, gate | None, pre_weight, post_rstd | None, pre_rstd); outputs = (dblock, dresidual,
+    dpost_weight | None, dgate | None, dpre_weight). dresidual may be dresidual_out. `workspace` is a uint8
+    CUDA tensor of at least `residual_norm_backward_workspace_bytes(...)` bytes; when omitted one is
+    allocated through torch's caching allocator for this call."""
+    dy, dresidual_out, block, residual_out, post_weight, gate, pre_weight, post_rstd, pre_rstd = inputs
+    dblock, dresidual, dpost_weight, dgate, dpre_weight = outputs
+    _check_matrix("dy", dy)
+    rows, cols = dy.shape
+    for name, t in (("dresidual_out", dresidual_out), ("block", block), ("residual_out", residual_out),
+                    ("dblock", dblock), ("dresidual", dresidual)):
+        if t is not None or name != "dresidual_out":
+            _check_like(name, t, dy, dy.dtype, (rows, cols))
+    for name, t, d in (("post_weight", post_weight, dpost_weight), ("gate", gate, dgate),
+                       ("pre_weight", pre_weight, dpre_weight)):
+        if (t is None) != (d is None):
+            raise ValueError(f"{name} and d{name} go together")
+        if t is not None or name == "pre_weight":
+            _check_like(name, t, dy, torch.float32, (cols,))
+            _check_like(f"d{name}", d, dy, torch.float32, (cols,))
+    if (post_weight is None) != (post_rstd is None):
+        raise ValueError("post_weight and post_rstd go together")
+    for name, t in (("post_rstd", post_rstd), ("pre_rstd", pre_rstd)):
+        if t is not None or name == "pre_rstd":
+            _check_like(name, t, dy, torch.float32, (rows,))
+    o = _opts(cluster_size, opts)
+    with torch.cuda.device(dy.device):
+        if workspace is None:
+            need = residual_norm_backward_workspace_bytes(rows, cols, dy.dtype, 0, o)
+            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dy.device)
+        if workspace.dim() != 1:
+            raise ValueError("workspace must have one dimension")
+        _check_like("workspace", workspace, dy, torch.uint8, workspace.shape)
+        N.check(N.load().credit_residual_norm_backward(
+            _ptr(dy), _ptr(dresidual_out), _ptr(block), _ptr(residual_out), _ptr(post_weight), _ptr(gate),
+            _ptr(pre_weight), _ptr(post_rstd), _ptr(pre_rstd), _ptr(dblock), _ptr(dresidual), _ptr(dpost_weight),
+            _ptr(dgate), _ptr(dpre_weight), rows, cols, residual_scale, _row_dtype(dy), _ref(o), _ptr(workspace),
+            workspace.numel(), _stream_ptr()))
+
+
+def _check_logits(name: str, t, dtype=None, shape=None) -> int:
+    """Row stride of a [rows, cols] matrix whose rows are contiguous, whole or as the leading columns of a
+    wider (padded) buffer."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got {t.dim()}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    rows, cols = t.shape
+    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+    return max(int(t.stride(0)), cols) if rows > 1 else cols
+
+
+def launch_token_logprobs_forward(inputs, outputs, cluster_size: int = 0, opts=None, temperature: float = 1.0) -> None:
+    """Log probabilities of given tokens under softmax(logits / temperature). inputs = (logits [rows, cols],
+    targets int64 [rows] | None), outputs = (logprob [rows] | None, stats [rows, 2], entropy [rows] | None,
+    top_logprob [rows, k] | None, top_index int64 [rows, k] | None). The logits may be the leading columns
+    of a wider buffer. A negative target is an ignored row."""
+    logits, targets = inputs
+    logprob, stats, entropy, top_logprob, top_index = outputs
+    stride = _check_logits("logits", logits)
+    rows, cols = logits.shape
+    if (targets is None) != (logprob is None):
+        raise ValueError("targets and logprob go together")
+    if targets is not None:
+        _check_like("targets", targets, logits, torch.int64, (rows,))
+        _check_like("logprob", logprob, logits, torch.float32, (rows,))
+    _check_like("stats", stats, logits, torch.float32, (rows, 2))
+    if entropy is not None:
+        _check_like("entropy", entropy, logits, torch.float32, (rows,))
+    if (top_logprob is None) != (top_index is None):
+        raise ValueError("top_logprob and top_index go together")
+    top_k = 0
+    if top_index is not None:
+        if top_index.dim() != 2:
+            raise ValueError("top_index must have two dimensions")
+        top_k = int(top_index.shape[1])
+        _check_like("top_index", top_index, logits, torch.int64, (rows, top_k))
+        _check_like("top_logprob", top_logprob, logits, torch.float32, (rows, top_k))
+    o = _opts(cluster_size, opts)
+    with torch.cuda.device(logits.device):
+        N.check(N.load().credit_token_logprobs_forward(
+            _ptr(logits), stride, _ptr(targets), _ptr(logprob), _ptr(stats), _ptr(entropy), _ptr(top_logprob),
+            _ptr(top_index), top_k, rows, cols, temperature, _row_dtype(logits), _ref(o), _stream_ptr()))
+
+
+def launch_token_logprobs_backward(inputs, outputs, cluster_size: int = 0, opts=None, temperature: float = 1.0) -> None:
+    """dlogits of sum(dlogprob * logprob) + sum(dentropy * entropy). inputs = (logits, targets, stats,
+    entropy | None, dlogprob, dentropy | None), outputs = (dlogits,), which may be the logits themselves."""
+    logits, targets, stats, entropy, dlogprob, dentropy = inputs
+    (dlogits,) = outputs
+    stride = _check_logits("logits", logits)
+    rows, cols = logits.shape
+    out_stride = _check_logits("dlogits", dlogits, logits.dtype, (rows, cols))
+    if dlogits.device != logits.device:
+        raise ValueError(f"dlogits must be on {logits.device}, got {dlogits.device}")
+    _check_like("targets", targets, logits, torch.int64, (rows,))
+    _check_like("stats", stats, logits, torch.float32, (rows, 2))
+    _check_like("dlogprob", dlogprob, logits, torch.float32, (rows,))
+    if dentropy is not None:
+        if entropy is None:
+            raise ValueError("dentropy needs the entropy of the forward pass")
+        _check_like("dentropy", dentropy, logits, torch.float32, (rows,))
+        _check_like("entropy", entropy, logits, torch.float32, (rows,))
+    o = _opts(cluster_size, opts)
+    with torch.cuda.device(logits.device):
+        N.check(N.load().credit_token_logprobs_backward(
+            _ptr(logits), stride, _ptr(targets), _ptr(stats), None if dentropy is None else _ptr(entropy),
+            _ptr(dlogprob), _ptr(dentropy), _ptr(dlogits), out_stride, rows, cols, temperature, _row_dtype(logits),
+            _ref(o), _stream_ptr()))
+
+
+def _check_teacher(index, value, logits) -> int:
+    if not isinstance(index, torch.Tensor) or index.dim() != 2:
+        raise ValueError("teacher_index must be a tensor of two dimensions")
+    top_k = int(index.shape[1])
+    _check_like("teacher_index", index, logits, torch.int64, (logits.shape[0], top_k))
+    _check_like("teacher_logprob", value, logits, torch.float32, (logits.shape[0], top_k))
+    return top_k
+
+
+def launch_distill_topk_forward(inputs, outputs, cluster_size: int = 0, opts=None, temperature: float = 1.0,
+                                tail: bool = True) -> None:
+    """KL(teacher || softmax(logits / temperature)) per row, the teacher given by its top log probabilities.
+    inputs = (logits [rows, cols], teacher_index int64 [rows, k], teacher_logprob [rows, k]), outputs =
+    (loss [rows], stats [rows, 6]). `tail`: what the list leaves of 1 is one more outcome; otherwise
+    the teacher is renormalised over its list. A negative index is an unused place."""
+    logits, index, value = inputs
+    loss, stats = outputs
+    stride = _check_logits("logits", logits)
+    rows, cols = logits.shape
+    top_k = _check_teacher(index, value, logits)
+    _check_like("loss", loss, logits, torch.float32, (rows,))
+    _check_like("stats", stats, logits, torch.float32, (rows, 6))
+    o = _opts(cluster_size, opts)
+    with torch.cuda.device(logits.device):
+        N.check(N.load().credit_distill_topk_forward(
+            _ptr(logits), stride, _ptr(index), _ptr(value), top_k, _ptr(loss), _ptr(stats), rows, cols, temperature,
+            1 if tail else 0, _row_dtype(logits), _ref(o), _stream_ptr()))
+
+
+def launch_distill_topk_backward(inputs, outputs, cluster_size: int = 0, opts=None, temperature: float = 1.0,
+                                 tail: bool = True) -> None:
+    """dlogits of sum(dloss * loss). inputs = (logits, teacher_index, teacher_logprob, stats, dloss), outputs =
+    (dlogits,), which may be the logits themselves. `stats` says whether the forward call had a tail;
+    `tail` is accepted for one signature with it."""
+    logits, index, value, stats, dloss = inputs
+    (dlogits,) = outputs
+    stride = _check_logits("logits", logits)
+    rows, cols = logits.shape
+    out_stride = _check_logits("dlogits", dlogits, logits.dtype, (rows, cols))
+    if dlogits.device != logits.device:
+        raise ValueError(f"dlogits must be on {logits.device}, got {dlogits.device}")
+    top_k = _check_teacher(index, value, logits)
+    _check_like("stats", stats, logits, torch.float32, (rows, 6))
+    _check_like("dloss", dloss, logits, torch.float32, (rows,))
+    o = _opts(cluster_size, opts)
+    with torch.cuda.device(logits.device):
+        N.check(N.load().credit_distill_topk_backward(
+            _ptr(logits), stride, _ptr(index), _ptr(value), top_k, _ptr(stats), _ptr(dloss), _ptr(dlogits), out_stride,
+            rows, cols, temperature, _row_dtype(logits), _ref(o), _stream_ptr()))
+
+
 # name -> (workload id, staged inputs, per-row input?, row-major outputs, per-row output?)
 _ROW_OPS = {
     "weighted_var_backward": (N.WL_WEIGHTED_VAR_BACKWARD, 3, False, 1, False),
@@ -258,15 +476,42 @@ NATIVE_LAUNCHERS = {
     "layernorm_backward": launch_layernorm_backward,
     "layernorm_backward_stats": launch_layernorm_backward_stats,
     "ffn_forward": launch_ffn_forward,
+    "residual_norm_forward": launch_residual_norm_forward,
+    "residual_norm_backward": launch_residual_norm_backward,
+    "token_logprobs_forward": launch_token_logprobs_forward,
+    "token_logprobs_backward": launch_token_logprobs_backward,
+    "distill_topk_forward": launch_distill_topk_forward,
+    "distill_topk_backward": launch_distill_topk_backward,
     **{name: _make_row_op_launcher(name) for name in _ROW_OPS},
 }
 
 
-def allocate_outputs(name: str, inputs: tuple[torch.Tensor, ...]) -> tuple[torch.Tensor, ...]:
-    """Output tensors for one call (reference: allocate_outputs, triton_kernels.py:403-414)."""
+def allocate_outputs(name: str, inputs: tuple[torch.Tensor, ...], top_k: int = 0,
+                     entropy: bool = True) -> tuple[torch.Tensor, ...]:
+    """Output tensors for one call (reference: allocate_outputs, triton_kernels.py:403-414). `top_k` and
+    `entropy` say which optional outputs token_logprobs_forward has; absent ones are None."""
     x = inputs[0]
     rows, cols = x.shape
     dev = x.device
+
+    def fp32(*shape):
+        return torch.empty(shape, device=dev, dtype=torch.float32)
+
+    if name == "residual_norm_forward":
+        return (torch.empty_like(x), torch.empty_like(x), None if inputs[2] is None else fp32(rows), fp32(rows))
+    if name == "residual_norm_backward":
+        return (torch.empty_like(x), torch.empty_like(x), None if inputs[4] is None else fp32(cols),
+                None if inputs[5] is None else fp32(cols), fp32(cols))
+    if name == "token_logprobs_forward":
+        return (None if inputs[1] is None else fp32(rows), fp32(rows, 2), fp32(rows) if entropy else None,
+                fp32(rows, top_k) if top_k else None,
+                torch.empty((rows, top_k), device=dev, dtype=torch.int64) if top_k else None)
+    if name == "distill_topk_forward":
+        return (fp32(rows), fp32(rows, 6))
+    if name in ("token_logprobs_backward", "distill_topk_backward"):
+        # rows as far apart as the logits': both then start at the same place between 16-byte boundaries
+        stride = max(int(x.stride(0)), cols)
+        return (torch.empty((rows, stride), device=dev, dtype=x.dtype)[:, :cols],)
     if name == "row_reduce":
         return (
             torch.empty(rows, device=dev, dtype=torch.float32),

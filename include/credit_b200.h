@@ -14,7 +14,8 @@
  *    src/workloads/layernorm_backward.cu:20-28). credit_last_error() gives the
  *    text for the calling thread's last failure.
  *  - Matrix pointers are caller-owned DEVICE pointers to row-major, densely
- *    packed [rows, cols] arrays on the current device. gamma/beta/dgamma/dbeta
+ *    packed [rows, cols] arrays on the current device (the logits of the
+ *    vocabulary-row entry points take a row stride). gamma/beta/dgamma/dbeta
  *    are always fp32 [cols]; per-row statistics are fp32 [rows].
  *  - Launches are asynchronous on `stream` (a cudaStream_t passed as void*; NULL
  *    is the default stream). No call allocates device memory or synchronises,
@@ -151,7 +152,8 @@ const char* credit_last_error(void);
 int credit_query_device(int device, credit_device_info* info);
 
 /* Reads (and optionally clears) the current device's status word: bit 0 = an
- * mbarrier wait timed out, bit 1 = a kernel refused its launch geometry.
+ * mbarrier wait timed out, bit 1 = a kernel refused its launch geometry, bit 2 = a
+ * token or teacher column index lies outside its row (that row's results are NaN).
  * Synchronises the device. Returns CREDIT_ERR_DEVICE_STATUS if any bit is set. */
 int credit_device_status(int* status_out, int reset);
 
@@ -286,6 +288,109 @@ int credit_layernorm_backward_stats_static(const void* x, const void* dy, const 
                                            const float* mean, const float* rstd, void* dx,
                                            float* dgamma, float* dbeta, int64_t rows, int64_t cols,
                                            int dtype, const credit_launch_opts* opts, void* stream);
+
+/* The end of a decoder --------------------------------------------------- */
+
+/* The norms after and before a block, fused with the block's gate and the scaled
+ * residual, for fp32 or bf16 [rows, cols] matrices and fp32 [cols] parameters:
+ *   n = block * rsqrt(mean(block^2) + eps)            (block itself without post_weight)
+ *   residual_out = residual_scale * residual + n * post_weight * gate
+ *   y = residual_out * rsqrt(mean(residual_out^2) + eps) * pre_weight
+ * post_weight (with post_rstd) and gate may be NULL: no post norm, no gate. y is
+ * computed from the unrounded sum. post_rstd and pre_rstd are fp32 [rows] outputs, what
+ * the backward call needs. residual_out may be residual or block, y may be block or
+ * residual, y and residual_out must differ. Rows up to 131072 columns (a row lives in the registers
+ * of a cluster); a wider row, or one wider than the asked cluster holds, gives
+ * CREDIT_ERR_UNSUPPORTED. Of the launch options, cluster_size only.
+ * No reference kernel exists for this; it stands beside credit_rmsnorm_forward. */
+int credit_residual_norm_forward(const void* block, const void* residual, const float* post_weight,
+                                 const float* gate, const float* pre_weight, void* residual_out, void* y,
+                                 float* post_rstd, float* pre_rstd, int64_t rows, int64_t cols,
+                                 float residual_scale, float eps, int dtype,
+                                 const credit_launch_opts* opts, void* stream);
+
+/* Its gradient: dblock and dresidual [rows, cols] and the fp32 [cols] sums over the rows
+ * dpost_weight, dgate (NULL exactly where the parameter is) and dpre_weight, which are
+ * written, not added to. dresidual_out is the gradient that reaches residual_out from
+ * elsewhere (NULL: none). residual_out and the rstd vectors are the forward call's.
+ * dresidual may be dresidual_out, dblock may be block or dy; dblock and dresidual must
+ * differ. The sums have a fixed order: equal calls give equal bits. `workspace` is 16-byte
+ * aligned device memory of at least the given bytes (for these rows, cols, dtype and
+ * options on the current device; with or without post norm); its contents need not be kept, and two calls
+ * that may overlap on the GPU need one each. rows = 0 writes zero sums. */
+size_t credit_residual_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int dtype,
+                                                     const credit_launch_opts* opts);
+int credit_residual_norm_backward(const void* dy, const void* dresidual_out, const void* block,
+                                  const void* residual_out, const float* post_weight, const float* gate,
+                                  const float* pre_weight, const float* post_rstd, const float* pre_rstd,
+                                  void* dblock, void* dresidual, float* dpost_weight, float* dgate,
+                                  float* dpre_weight, int64_t rows, int64_t cols, float residual_scale,
+                                  int dtype, const credit_launch_opts* opts, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens, with the entropy and the top alternatives of each
+ * row of fp32 or bf16 logits. Row r starts at logits + r * row_stride elements (row_stride
+ * >= cols; a padded vocabulary); columns behind `cols` are never read or written. With
+ * z = logits / temperature and p = softmax(z), all outputs fp32 but top_index:
+ *   logprob[r] = log p[targets[r]]
+ *   stats[r]   = (max of the row's LOGITS, log sum exp(z - max z)): what the backward call
+ *                needs; max / temperature + log sum is the row's log-sum-exp
+ *   entropy[r] = -sum p log p                                     (NULL: not computed)
+ *   top_logprob[r, 0..top_k), top_index[r, ...]: the top_k (0...128) largest logits, descending, ties by
+ *                ascending column
+ * targets and logprob may both be NULL: alternatives or entropy alone.
+ *   - A negative target marks an ignored row: its logits are not read, logprob, stats and
+ *     entropy are 0, alternatives absent. A target >= cols sets bit 2 of the device status
+ *     and gives NaN.
+ *   - -inf is a masked logit: probability 0 and never an alternative. Places without an
+ *     alternative hold index -1 and -inf. A row of -inf only has logprob -inf, entropy 0,
+ *     stats (-inf, 0).
+ *   - A row that holds NaN or +inf has NaN for its real results; as alternatives NaN ranks above
+ *     +inf.
+ * Of the launch options, cluster_size only (CTAs per row). No reference kernel exists;
+ * it stands beside the softmax-logits backward (softmax_logits_backward.cu:410). */
+int credit_token_logprobs_forward(const void* logits, int64_t row_stride, const int64_t* targets,
+                                  float* logprob, float* stats, float* entropy, float* top_logprob,
+                                  int64_t* top_index, int top_k, int64_t rows, int64_t cols,
+                                  float temperature, int dtype, const credit_launch_opts* opts,
+                                  void* stream);
+
+/* dlogits of sum_r dlogprob[r] * logprob[r] + dentropy[r] * entropy[r]; dentropy (with
+ * entropy) may be NULL. dlogits has its own row stride and may be the logits themselves;
+ * otherwise the two must not overlap. Ignored rows and rows of -inf only get zeros. */
+int credit_token_logprobs_backward(const void* logits, int64_t row_stride, const int64_t* targets,
+                                   const float* stats, const float* entropy, const float* dlogprob,
+                                   const float* dentropy, void* dlogits, int64_t dlogits_row_stride,
+                                   int64_t rows, int64_t cols, float temperature, int dtype,
+                                   const credit_launch_opts* opts, void* stream);
+
+/* Distillation from a teacher's top logits: per row KL(teacher || student), the student
+ * being softmax(logits / temperature) and the teacher a list of top_k (1...128) columns
+ * teacher_index [rows, top_k] with fp32 teacher_logprob [rows, top_k], as
+ * credit_token_logprobs_forward lists them (any order).
+ *   tail = 0: the teacher is softmax(teacher_logprob) over its list (raw logits do as well);
+ *   tail = 1: teacher_logprob are log probabilities, and what they leave of 1 is one more
+ *             outcome that is compared with the student's mass outside the list.
+ * loss is fp32 [rows]; stats fp32 [rows, 6] is the state the backward call needs.
+ *   - A negative index marks an unused place. A row without a used place (or, with tail = 0,
+ *     without teacher mass) has loss 0 and no gradient, and its logits are not read. An
+ *     index >= cols sets bit 2 of the device status and gives NaN.
+ *   - A column listed twice counts with the sum of its weights' terms in the loss, and once
+ *     in the student's mass.
+ *   - With tail = 1, when the student has nothing left outside the list, or the list sums to
+ *     more than 1, the teacher is renormalised over the list.
+ *   - Masked (-inf) logits under teacher mass give loss +inf and a finite gradient; a row of
+ *     -inf only has no gradient; NaN or +inf in a row gives NaN.
+ * dlogits and its stride as in credit_token_logprobs_backward. */
+int credit_distill_topk_forward(const void* logits, int64_t row_stride, const int64_t* teacher_index,
+                                const float* teacher_logprob, int top_k, float* loss, float* stats,
+                                int64_t rows, int64_t cols, float temperature, int tail, int dtype,
+                                const credit_launch_opts* opts, void* stream);
+int credit_distill_topk_backward(const void* logits, int64_t row_stride, const int64_t* teacher_index,
+                                 const float* teacher_logprob, int top_k, const float* stats,
+                                 const float* dloss, void* dlogits, int64_t dlogits_row_stride,
+                                 int64_t rows, int64_t cols, float temperature, int dtype,
+                                 const credit_launch_opts* opts, void* stream);
 
 /* Host-buffer entry points ----------------------------------------------- */
 
