@@ -112,7 +112,7 @@ __device__ __forceinline__ void load_list(const DistillArgs& a, int64_t row, Tea
 // forward: one cluster per row, the row read once
 // ---------------------------------------------------------------------------
 template <typename T, bool TAIL>
-__global__ void __launch_bounds__(kThreads) distill_topk_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) distill_topk_kernel(const DistillArgs a) {
     __shared__ SoftmaxRecord warp_records[kThreads / 32];
     __shared__ SoftmaxRecord records[kMaxClusterSize];
     __shared__ TeacherList list;
@@ -174,26 +174,24 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(const DistillArg
             if (bits >> j & 1u) y[j] = -CUDART_INF_F;
         v = Vec<T>::pack(y);
     };
-    stream_slice<T, kThreads, kUnroll>(
-        span,
-        [&](uint4 (&v)[kUnroll], int first, int) {
-            if (TAIL) {
+    const float edge = edge_element(span);
+    stream_chunks<T, kThreads, kUnroll>(span, 0, chunks_of<T, kThreads, kUnroll>(span), [&](uint4 (&v)[kUnroll], int first) {
+        if (TAIL) {
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
-                    const int p = (first + u * kThreads) * E;
-                    const uint32_t bits = p < span.nvec * E ? bitmap[p >> 5] >> (p & 31) & ((1u << E) - 1u) : 0u;
-                    if (bits != 0) hide(v[u], bits);
-                }
+            for (int u = 0; u < kUnroll; ++u) {
+                const int p = (first + u * kThreads) * E;
+                const uint32_t bits = p < span.nvec * E ? bitmap[p >> 5] >> (p & 31) & ((1u << E) - 1u) : 0u;
+                if (bits != 0) hide(v[u], bits);
             }
-            add(v);
-        },
-        [&](uint4 (&v)[1]) {
-            if (TAIL && tid < span.edges) {
-                const int p = span.nvec * E + tid;
-                if (bitmap[p >> 5] >> (p & 31) & 1u) v[0] = masked_vec<T>();
-            }
-            add(v);
-        });
+        }
+        add(v);
+    });
+    if (span.edges > 0) {
+        const int p = span.nvec * E + tid;
+        const bool hidden = TAIL && tid < span.edges && (bitmap[p >> 5] >> (p & 31) & 1u) != 0;
+        uint4 v[1] = {Vec<T>::single(hidden ? -CUDART_INF_F : edge)};
+        add(v);
+    }
     rec = cta_record<kThreads>(rec, warp_records, k2);
     cluster_wait_acquire();
     if (nranks > 1) {
@@ -212,7 +210,11 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(const DistillArg
     if (tid < kMaxList) student[tid] = listed;
     __syncthreads();
     if (tid >= 32) return;
-    for (uint32_t r = 1; r < nranks; ++r) rec = merge_records(rec, records[r], k2);
+    if (nranks > 1) {
+        if (tid == 0) records[0] = rec;
+        __syncwarp();
+        rec = warp_record<kMaxClusterSize>(tid < static_cast<int>(nranks) ? records[tid] : empty_record(), k2);
+    }
     SoftmaxRecord all = rec;   // with a tail `rec` covers the columns outside the list
     if (TAIL) {
         // the listed columns, each once: a repeated column counts where it appears first
@@ -229,16 +231,19 @@ __global__ void __launch_bounds__(kThreads) distill_topk_kernel(const DistillArg
         }
         SoftmaxRecord mine = empty_record();
         mine.m = warp_max_nan(top);
-        const float base = mine.m == -CUDART_INF_F ? 0.0f : mine.m;
+        // relative to the base of this maximum, as the row's sums are
+        const bool by_base = has_base(mine.m, k2);
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) mine.s += ex2_approx((y[i] - base) * k2);
+        for (int i = 0; i < kPerLane; ++i)
+            if (y[i] != -CUDART_INF_F)
+                mine.s += ex2_approx(by_base ? fmaf(y[i], k2, -base_of(mine.m, k2)) : (y[i] - mine.m) * k2);
         mine.s = warp_sum(mine.s);
         all = merge_records(rec, mine, k2);
     }
     const bool broken = is_broken(all.m) || list.bad;
     const bool empty = all.m == -CUDART_INF_F, no_tail = rec.m == -CUDART_INF_F;
-    const float log_sum = empty ? 0.0f : logf(all.s);
-    const float tail_log_sum = no_tail ? 0.0f : logf(rec.s);
+    const float log_sum = empty ? 0.0f : log_sum_of(all, k2);
+    const float tail_log_sum = no_tail ? 0.0f : log_sum_of(rec, k2);
     // the teacher: always a distribution. Without anything left outside the student's list, or with a
     // list of more than 1, it is renormalised over the list.
     float log_norm = list.log_norm, rest = 0.0f;

@@ -40,7 +40,7 @@ struct LogprobArgs {
 // forward: one cluster per row, the row read once
 // ---------------------------------------------------------------------------
 template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const LogprobArgs a) {
     __shared__ SoftmaxRecord warp_records[kThreads / 32];
     __shared__ SoftmaxRecord records[kMaxClusterSize];   // rank 0: one per CTA
     __shared__ float row_max, row_log_sum;
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobA
             return;
         }
     }
-    if (!TOP) cluster_arrive_release();   // "this CTA runs": its shared memory may be written from now on
+    cluster_arrive_release();   // "this CTA runs": its shared memory may be written from now on
     float picked = CUDART_NAN_F;
     if (a.targets != nullptr && rank == 0 && tid == 0) {
         if (target < a.cols) {
@@ -85,91 +85,79 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const LogprobA
     const int local = max(0, min(a.slice, a.cols - start));
     const RowSpan<T> span(x, start, local);
     const float k2 = a.inv_t * kLog2e;
+    const float edge = edge_element(span);
     SoftmaxRecord rec = empty_record();
     TopCollector<T> collector(t, a.top_k);
-    int next_tighten = 4;
-    constexpr int kStride = kThreads * Vec<T>::kElems;
-    stream_slice<T, kThreads, kUnroll>(
-        span,
-        [&](const uint4 (&v)[kUnroll], int first, int it) {
+    const int chunks = chunks_of<T, kThreads, kUnroll>(span);
+    int from = 0, to = TOP ? 1 : chunks;
+    do {
+        stream_chunks<T, kThreads, kUnroll>(span, from, min(to, chunks), [&](const uint4 (&v)[kUnroll], int first) {
             float part[kUnroll];
             const float top = chunk_max<T>(v, part);
             if (TOP) {
+                constexpr int kStride = kThreads * Vec<T>::kElems;
                 const int column = span.vector_column(first);
-                if (it == 0) {
-                    collector.first_threshold(v, part, top, column, kStride);
-                } else if (it == next_tighten) {
-                    collector.tighten();
-                    next_tighten *= 4;
-                }
-                collector.offer_chunk(v, part, top, column, kStride);
+                if (from == 0) collector.first_threshold(v, part, top, column, kStride);
+                collector.note_chunk(part, top, first, column, kStride);
             }
             accumulate<T, kUnroll, ENTROPY>(v, top, k2, rec);
-        },
-        [&](const uint4 (&v)[1]) {
-            const float top = Vec<T>::max(v[0]);
-            if (TOP) {
-                if (span.nvec == 0) __syncthreads();   // the buffer's first use
-                if (tid < span.edges) {
-                    float e[Vec<T>::kElems];
-                    Vec<T>::unpack(v[0], e);
-                    collector.offer(e[0], span.start + span.edge_offset(tid));
-                }
-            }
-            accumulate<T, 1, ENTROPY>(v, top, k2, rec);
         });
+        from = to;
+        to *= 4;
+        if (TOP && from < chunks) collector.tighten(span);
+    } while (from < chunks);
+    if (span.edges > 0) {
+        if (TOP) {
+            if (chunks == 0) __syncthreads();   // the buffer's first use
+            if (tid < span.edges) collector.offer(edge, span.start + span.edge_offset(tid));
+        }
+        const uint4 v[1] = {Vec<T>::single(edge)};
+        accumulate<T, 1, ENTROPY>(v, edge, k2, rec);
+    }
 
     rec = cta_record<kThreads>(rec, warp_records, k2);
     if (TOP) collector.finish(span);
+    cluster_wait_acquire();
     if (nranks > 1) {
-        if (TOP) cluster_arrive_release();   // this CTA's list is ready and its buffer may be written
-        cluster_wait_acquire();
-        if (rank != 0) {
-            if (tid == 0) {
-                const uint32_t to = map_to_rank(smem_u32(&records[rank]), 0);
-                st_cluster_f32(to, rec.m);
-                st_cluster_f32(to + 4, rec.s);
-                st_cluster_f32(to + 8, rec.e);
-            }
-            if (TOP && tid < a.top_k)
-                st_cluster_u64(map_to_rank(smem_u32(&t.keys[rank * a.top_k + tid]), 0), tid < t.fill ? t.keys[tid] : 0);
-        } else if (TOP && tid < a.top_k && tid >= t.fill) {
-            t.keys[tid] = 0;
+        // rank 0 gathers the records, and the lists behind its own buffer
+        unsigned long long* gathered = reinterpret_cast<unsigned long long*>(&t + 1);
+        if (rank != 0 && tid == 0) {
+            const uint32_t to0 = map_to_rank(smem_u32(&records[rank]), 0);
+            st_cluster_f32(to0, rec.m);
+            st_cluster_f32(to0 + 4, rec.s);
+            st_cluster_f32(to0 + 8, rec.e);
         }
+        if (TOP && tid < a.top_k)
+            st_cluster_u64(map_to_rank(smem_u32(&gathered[rank * a.top_k + tid]), 0), tid < t.fill ? t.keys[tid] : 0);
         cluster_sync_all();
         if (rank != 0) return;
-        if (TOP) keep_largest(t, static_cast<int>(nranks) * a.top_k, a.top_k);
-    } else if (!TOP) {
-        cluster_wait_acquire();
+        if (TOP) merge_lists(t, gathered, static_cast<int>(nranks), a.top_k);
+        if (tid < 32) {
+            if (tid == 0) records[0] = rec;
+            __syncwarp();
+            rec = warp_record<kMaxClusterSize>(tid < static_cast<int>(nranks) ? records[tid] : empty_record(), k2);
+        }
     }
 
     if (tid == 0) {
-        for (uint32_t r = 1; r < nranks; ++r) rec = merge_records(rec, records[r], k2);
         const bool broken = is_broken(rec.m), empty = rec.m == -CUDART_INF_F;
-        const float log_sum = broken ? CUDART_NAN_F : (empty ? 0.0f : logf(rec.s));
+        const float log_sum = broken ? CUDART_NAN_F : (empty ? 0.0f : log_sum_of(rec, k2));
         row_max = rec.m;
         row_log_sum = log_sum;
         a.stats[2 * row] = rec.m;
         a.stats[2 * row + 1] = log_sum;
         if (a.targets != nullptr)
             a.logprob[row] = empty && target < a.cols ? -CUDART_INF_F : (picked - rec.m) * a.inv_t - log_sum;
-        if (ENTROPY) a.entropy[row] = broken ? CUDART_NAN_F : (empty ? 0.0f : log_sum - kLn2 * (rec.e / rec.s));
+        if (ENTROPY) a.entropy[row] = broken ? CUDART_NAN_F : (empty ? 0.0f : logf(rec.s) - kLn2 * (rec.e / rec.s));
     }
     if (TOP) {
         __syncthreads();
-        const int n = min(t.fill, a.top_k);
         if (tid < a.top_k) {
-            const int64_t base = row * a.top_k;
-            if (tid < n) {
-                const uint64_t key = t.keys[tid];
-                int place = 0;
-                for (int i = 0; i < n; ++i) place += t.keys[i] > key;
-                a.top_logprob[base + place] = (key_value(key) - row_max) * a.inv_t - row_log_sum;
-                a.top_index[base + place] = key_column(key);
-            } else {
-                a.top_logprob[base + tid] = -CUDART_INF_F;
-                a.top_index[base + tid] = -1;
-            }
+            const int64_t at = row * a.top_k + tid;
+            const bool present = tid < t.fill;
+            const uint64_t key = present ? t.keys[tid] : 0;
+            a.top_logprob[at] = present ? (key_value(key) - row_max) * a.inv_t - row_log_sum : -CUDART_INF_F;
+            a.top_index[at] = present ? key_column(key) : -1;
         }
     }
 }
@@ -343,7 +331,9 @@ int forward(const void* logits, int64_t ld, const int64_t* targets, float* logpr
     rc = prepare_kernel(ctx, func);
     if (rc != CREDIT_OK) return rc;
     void* args[] = {&a};
-    return launch_kernel(func, rows * cluster, kThreads, cluster, top ? static_cast<int>(sizeof(TopBuffer)) : 0, stream, args);
+    // the candidates, and in a cluster the lists that rank 0 gathers
+    const size_t smem = top ? sizeof(TopBuffer) + (cluster > 1 ? sizeof(uint64_t) * cluster * top_k : 0) : 0;
+    return launch_kernel(func, rows * cluster, kThreads, cluster, static_cast<int>(smem), stream, args);
 }
 
 int backward(const void* logits, int64_t ld, const int64_t* targets, const float* stats, const float* entropy,

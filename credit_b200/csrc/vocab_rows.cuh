@@ -1,14 +1,18 @@
 // Building blocks of the kernels that read a row of logits once (token_logprobs.cu,
 // distill_topk.cu): the 16-byte-vector view of a row slice of any alignment, the chunked streaming
-// loop, and the softmax record of one pass,
-//     m = max x,  s = sum exp(k (x - m)),  e = sum exp(k (x - m)) * k (x - m),   k = 1 / temperature,
-// in 32 bits. Differences x - m are taken before the scaling, so rows far from zero (and rows whose
-// every logit is the type's lowest value) lose nothing; the exponential is ex2.approx (relative
-// error 2^-22) of the difference in base-2 units, and so is e.
+// loop, and the softmax record of one pass.
 //
-// -inf is a masked logit: it adds nothing (differences are clamped at -200, where ex2 gives 0, before
-// they are multiplied by that 0). A NaN makes m NaN (max.NaN), +inf makes it +inf; both are turned
-// into NaN results when the row is finished.
+// With k2 = log2(e) / temperature and a base b = m k2 rounded to fp32, m the maximum so far,
+//     s = sum 2^(x k2 - b),   e = sum 2^(x k2 - b) (x k2 - b)        in 32 bits.
+// x k2 - b is one fused multiply-add: exact products, so rows far from zero lose nothing; what the rounding
+// of b shifts (at most half an ulp of b) is known and taken out again when the row is finished:
+//     log sum exp((x - m) / T) = ln s - ln2 (m k2 - b),   entropy = ln s - ln2 e / s.
+// The exponential is ex2.approx (relative error 2^-22).
+//
+// -inf is a masked logit: 2^-inf adds nothing, and where it would meet e it is replaced by -1e30. Rows
+// whose maximum is itself near the type's lowest value (a mask of finite values that leaves nothing) or
+// whose base overflows take the same sums from differences x - m. A NaN makes m NaN (max.NaN), +inf makes
+// it +inf; both are turned into NaN results when the row is finished.
 #pragma once
 
 #include <math_constants.h>
@@ -19,6 +23,8 @@ namespace credit {
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowLogit = -1e29f;   // rows whose maximum is below it go by differences
+constexpr float kDeepLogit = -1e30f;  // stands for -inf where a product with 0 follows
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -42,6 +48,17 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
     return v;
 }
 
+// Monotone image of a float: unsigned order is the order of the values, -0 equal to +0, NaN above +inf.
+__device__ __forceinline__ uint32_t ordered_image(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);   // -0 + 0 = +0
+    if (x != x) return 0xffffffffu;
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+__device__ __forceinline__ float image_value(uint32_t k) {
+    return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
+}
+
 // ---------------------------------------------------------------------------
 // 16-byte vectors
 // ---------------------------------------------------------------------------
@@ -63,6 +80,14 @@ struct Vec<float> {
         float x[4];
         unpack(v, x);
         return max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
+    }
+    // -inf (and anything below kDeepLogit) raised to kDeepLogit
+    __device__ __forceinline__ static uint4 deep(const uint4& v) {
+        float x[4];
+        unpack(v, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = fmaxf(x[i], kDeepLogit);
+        return pack(x);
     }
     __device__ __forceinline__ static uint4 single(float x) {
         return make_uint4(__float_as_uint(x), kMaskedWord, kMaskedWord, kMaskedWord);
@@ -90,6 +115,15 @@ struct Vec<__nv_bfloat16> {
     __device__ __forceinline__ static uint32_t max2(uint32_t a, uint32_t b) {
         uint32_t r;
         asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    __device__ __forceinline__ static uint4 deep(const uint4& v) {
+        constexpr uint32_t kDeepWord = 0xf149f149u;   // -0.995e30 twice
+        uint4 r;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r.x) : "r"(v.x), "r"(kDeepWord));
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r.y) : "r"(v.y), "r"(kDeepWord));
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r.z) : "r"(v.z), "r"(kDeepWord));
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r.w) : "r"(v.w), "r"(kDeepWord));
         return r;
     }
     __device__ __forceinline__ static float max(const uint4& v) {
@@ -136,41 +170,46 @@ struct RowSpan {
     __device__ __forceinline__ int vector_column(int v) const { return start + head + v * Vec<T>::kElems; }
 };
 
-// Calls f(v, first_vec, it) for chunks of U vectors a thread (vector first_vec + u * THREADS is v[u];
-// places past the end hold -inf) and once more with it = number of chunks for the edge elements,
-// if there are any, as f's `edge` call: v[0] holds edge element threadIdx.x alone. Every thread of
-// the CTA makes the same calls, so f may synchronise. The next chunk is in flight while f runs.
-template <typename T, int THREADS, int U, typename F, typename G>
-__device__ __forceinline__ void stream_slice(const RowSpan<T>& s, F&& f, G&& edge) {
+template <typename T, int THREADS, int U>
+__device__ __forceinline__ int chunks_of(const RowSpan<T>& s) {
+    return (s.nvec + THREADS * U - 1) / (THREADS * U);
+}
+
+// Calls f(v, first) for chunks [from, to) of U vectors a thread (vector first + u * THREADS is v[u];
+// places past the end hold -inf). Every thread of the CTA makes the same calls, so f may synchronise. The
+// next chunk is in flight while f runs.
+template <typename T, int THREADS, int U, typename F>
+__device__ __forceinline__ void stream_chunks(const RowSpan<T>& s, int from, int to, F&& f) {
     constexpr int kPerChunk = THREADS * U;
-    const int chunks = (s.nvec + kPerChunk - 1) / kPerChunk;
     const uint4* base = s.vectors();
-    uint4 next[U];
-    auto fetch = [&](int it) {
+    auto fetch = [&](int it, uint4 (&v)[U]) {
         const int i0 = it * kPerChunk + static_cast<int>(threadIdx.x);
         if ((it + 1) * kPerChunk <= s.nvec) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) next[u] = load_stream(base + i0 + u * THREADS);
+            for (int u = 0; u < U; ++u) v[u] = load_stream(base + i0 + u * THREADS);
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                next[u] = i0 + u * THREADS < s.nvec ? load_stream(base + i0 + u * THREADS) : masked_vec<T>();
+                v[u] = i0 + u * THREADS < s.nvec ? load_stream(base + i0 + u * THREADS) : masked_vec<T>();
         }
     };
-    float lone = -CUDART_INF_F;
-    if (static_cast<int>(threadIdx.x) < s.edges) lone = Vec<T>::load(s.first + s.edge_offset(threadIdx.x));
-    if (chunks > 0) fetch(0);
-    for (int it = 0; it < chunks; ++it) {
-        uint4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = next[u];
-        if (it + 1 < chunks) fetch(it + 1);
-        f(v, it * kPerChunk + static_cast<int>(threadIdx.x), it);
+    uint4 a[U], b[U];
+    if (from < to) fetch(from, a);
+#pragma unroll 1
+    for (int it = from; it < to; it += 2) {
+        if (it + 1 < to) fetch(it + 1, b);
+        f(a, it * kPerChunk + static_cast<int>(threadIdx.x));
+        if (it + 1 >= to) break;
+        if (it + 2 < to) fetch(it + 2, a);
+        f(b, (it + 1) * kPerChunk + static_cast<int>(threadIdx.x));
     }
-    if (s.edges > 0) {
-        uint4 v[1] = {Vec<T>::single(lone)};
-        edge(v);
-    }
+}
+
+// Edge element threadIdx.x of the slice (load it early, before the chunks), -inf when there is none.
+template <typename T>
+__device__ __forceinline__ float edge_element(const RowSpan<T>& s) {
+    const int i = static_cast<int>(threadIdx.x);
+    return i < s.edges ? Vec<T>::load(s.first + s.edge_offset(i)) : -CUDART_INF_F;
 }
 
 // ---------------------------------------------------------------------------
@@ -178,17 +217,25 @@ __device__ __forceinline__ void stream_slice(const RowSpan<T>& s, F&& f, G&& edg
 // ---------------------------------------------------------------------------
 struct SoftmaxRecord {
     float m;   // maximum logit
-    float s;   // sum of ex2(k2 (x - m)), k2 = log2(e) / temperature
-    float e;   // sum of the same times k2 (x - m)
+    float s, e;
 };
 
 __device__ __forceinline__ SoftmaxRecord empty_record() { return {-CUDART_INF_F, 0.0f, 0.0f}; }
 
+__device__ __forceinline__ float base_of(float m, float k2) { return __fmul_rn(m, k2); }
+
+// (k2 below 1e-20: temperatures at which kDeepLogit would not be far away)
+__device__ __forceinline__ bool has_base(float m, float k2) {
+    return m > kLowLogit && fabsf(base_of(m, k2)) < CUDART_INF_F && k2 > 1e-20f;
+}
+
 // Moves a record to a maximum that is at least its own.
 __device__ __forceinline__ void raise_maximum(SoftmaxRecord& a, float m, float k2) {
-    const float d = fmaxf((a.m - m) * k2, -200.0f);   // -200 too for a.m = m = -inf (s = e = 0 there)
-    const float r = a.m == m ? 1.0f : ex2_approx(d);
-    a.e = a.m == m ? a.e : (a.e + a.s * d) * r;
+    if (a.m == m) return;
+    float d = has_base(a.m, k2) && has_base(m, k2) ? __fsub_rn(base_of(a.m, k2), base_of(m, k2)) : (a.m - m) * k2;
+    d = fmaxf(d, -200.0f);   // 2^-200 is 0 here; also for a.m = -inf, where s = e = 0
+    const float r = ex2_approx(d);
+    a.e = (a.e + a.s * d) * r;
     a.s *= r;
     a.m = m;
 }
@@ -200,26 +247,47 @@ __device__ __forceinline__ SoftmaxRecord merge_records(SoftmaxRecord a, SoftmaxR
     return {m, a.s + b.s, a.e + b.e};
 }
 
+// ln of the sum relative to the maximum.
+__device__ __forceinline__ float log_sum_of(const SoftmaxRecord& a, float k2) {
+    const float shift = has_base(a.m, k2) ? fmaf(a.m, k2, -base_of(a.m, k2)) : 0.0f;
+    return logf(a.s) - kLn2 * shift;
+}
+
 // Adds U vectors whose maximum is `top`. The rescaling is rare: a thread's maximum settles after a
 // few chunks.
 template <typename T, int U, bool ENTROPY>
 __device__ __forceinline__ void accumulate(const uint4 (&v)[U], float top, float k2, SoftmaxRecord& a) {
     constexpr int E = Vec<T>::kElems;
     if (!(top <= a.m)) raise_maximum(a, max_nan(a.m, top), k2);   // a NaN stays
-    const float base = a.m == -CUDART_INF_F ? 0.0f : a.m;   // nothing but masked logits yet: ex2(-inf) = 0
-    const float2 minus = make_float2(-base, -base), scale = make_float2(k2, k2);
+    if (!has_base(a.m, k2)) {
+        if (a.m == -CUDART_INF_F) return;   // nothing but masked logits yet
+#pragma unroll 1
+        for (int u = 0; u < U; ++u) {
+            float x[E];
+            uint4 w = v[0];
+#pragma unroll
+            for (int i = 1; i < U; ++i)
+                if (i == u) w = v[i];
+            Vec<T>::unpack(w, x);
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                const float d = fmaxf((x[j] - a.m) * k2, -200.0f), p = ex2_approx(d);
+                a.s += p;
+                a.e = fmaf(p, d, a.e);
+            }
+        }
+        return;
+    }
+    const float base = -base_of(a.m, k2);
+    const float2 minus = make_float2(base, base), scale = make_float2(k2, k2);
     float2 s[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}}, e[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         float x[E];
-        Vec<T>::unpack(v[u], x);
+        Vec<T>::unpack(ENTROPY ? Vec<T>::deep(v[u]) : v[u], x);
 #pragma unroll
         for (int j = 0; j < E; j += 2) {
-            float2 d = __fmul2_rn(__fadd2_rn(make_float2(x[j], x[j + 1]), minus), scale);
-            if (ENTROPY) {
-                d.x = fmaxf(d.x, -200.0f);
-                d.y = fmaxf(d.y, -200.0f);
-            }
+            const float2 d = __ffma2_rn(make_float2(x[j], x[j + 1]), scale, minus);
             const float2 p = make_float2(ex2_approx(d.x), ex2_approx(d.y));
             const int w = (j / 2) & 1;
             s[w] = __fadd2_rn(s[w], p);
@@ -241,25 +309,32 @@ __device__ __forceinline__ float chunk_max(const uint4 (&v)[U], float (&part)[U]
     return top;
 }
 
-// The CTA's record, in every thread of warp 0 (the other warps get their own warp's). `slots` holds one
+// Records of the first COUNT lanes (a power of two; the others must hold empty ones) in every lane: one maximum
+// over the warp, one rescaling, plain sums.
+template <int COUNT>
+__device__ __forceinline__ SoftmaxRecord warp_record(SoftmaxRecord a, float k2) {
+    const float m = image_value(__reduce_max_sync(0xffffffffu, ordered_image(a.m)));
+    raise_maximum(a, m, k2);
+#pragma unroll
+    for (int o = COUNT / 2; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.e += __shfl_xor_sync(0xffffffffu, a.e, o);
+    }
+    a.s = __shfl_sync(0xffffffffu, a.s, 0);
+    a.e = __shfl_sync(0xffffffffu, a.e, 0);
+    return a;
+}
+
+// The CTA's record, in every lane of warp 0 (the other warps get their own warp's). `slots` holds one
 // record per warp. One barrier.
 template <int THREADS>
 __device__ __forceinline__ SoftmaxRecord cta_record(SoftmaxRecord a, SoftmaxRecord* slots, float k2) {
+    constexpr int kWarps = THREADS / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        SoftmaxRecord b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        b.e = __shfl_xor_sync(0xffffffffu, a.e, o);
-        a = merge_records(a, b, k2);
-    }
+    a = warp_record<32>(a, k2);
     if (lane == 0) slots[warp] = a;
     __syncthreads();
-    if (warp == 0) {
-        a = slots[0];
-        for (int w = 1; w < THREADS / 32; ++w) a = merge_records(a, slots[w], k2);
-    }
+    if (warp == 0) a = warp_record<kWarps>(lane < kWarps ? slots[lane] : empty_record(), k2);
     return a;
 }
 

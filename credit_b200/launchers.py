@@ -204,16 +204,39 @@ def launch_ffn_forward(inputs, outputs, cluster_size: int = 0, opts=None, eps: f
             workspace.data_ptr(), workspace.numel(), _stream_ptr()))
 
 
-def _check_like(name: str, t, x: torch.Tensor, dtype, shape) -> None:
-    """A tensor that must lie beside `x`: the checks of `_check_matrix` and the same device."""
-    _check_matrix(name, t, dtype, shape)
-    if t.device != x.device:
-        raise ValueError(f"{name} must be on {x.device}, got {t.device}")
+def _check_like(name: str, t, device: torch.device, dtype, shape) -> "int | None":
+    """The checks of `_check_matrix` and that the tensor lies on `device`; returns its address (NULL when it
+    is empty). What is in order costs a handful of attribute reads: small calls are bound by their host side."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device
+            and t.is_contiguous()):
+        _check_matrix(name, t, dtype, shape)
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    return t.data_ptr() or None
 
 
-def _ptr(t) -> "int | None":
-    """Device address, or NULL for an absent or empty tensor."""
-    return None if t is None or t.numel() == 0 else t.data_ptr()
+def _check_optional(name: str, t, device: torch.device, dtype, shape) -> "int | None":
+    return None if t is None else _check_like(name, t, device, dtype, shape)
+
+
+def _options(cluster_size: int, opts):
+    return None if not cluster_size and opts is None else _ref(_opts(cluster_size, opts))
+
+
+# The current stream's address without a Stream object around it (0.1 us instead of 2.2 us a call).
+_current_stream_ptr = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(entry, device: torch.device, *args) -> None:
+    """Runs a C entry point with `device` current, on that device's current stream."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = entry(*args, _current_stream_ptr(index))
+    else:
+        with torch.cuda.device(device):
+            status = entry(*args, _current_stream_ptr(index))
+    if status:
+        N.check(status)
 
 
 def launch_residual_norm_forward(inputs, outputs, cluster_size: int = 0, opts=None, residual_scale: float = 1.0,
@@ -228,22 +251,19 @@ def launch_residual_norm_forward(inputs, outputs, cluster_size: int = 0, opts=No
     block, residual, post_weight, gate, pre_weight = inputs
     residual_out, y, post_rstd, pre_rstd = outputs
     _check_matrix("block", block)
-    rows, cols = block.shape
-    for name, t in (("residual", residual), ("residual_out", residual_out), ("y", y)):
-        _check_like(name, t, block, block.dtype, (rows, cols))
-    for name, t in (("post_weight", post_weight), ("gate", gate), ("pre_weight", pre_weight)):
-        if t is not None or name == "pre_weight":
-            _check_like(name, t, block, torch.float32, (cols,))
+    rows, cols = shape = block.shape
+    device, dtype, f32 = block.device, block.dtype, torch.float32
     if (post_weight is None) != (post_rstd is None):
         raise ValueError("post_weight and post_rstd go together")
-    for name, t in (("post_rstd", post_rstd), ("pre_rstd", pre_rstd)):
-        if t is not None or name == "pre_rstd":
-            _check_like(name, t, block, torch.float32, (rows,))
-    o = _opts(cluster_size, opts)
-    with torch.cuda.device(block.device):
-        N.check(N.load().credit_residual_norm_forward(
-            _ptr(block), _ptr(residual), _ptr(post_weight), _ptr(gate), _ptr(pre_weight), _ptr(residual_out), _ptr(y),
-            _ptr(post_rstd), _ptr(pre_rstd), rows, cols, residual_scale, eps, _row_dtype(block), _ref(o), _stream_ptr()))
+    _call(N.load().credit_residual_norm_forward, device, block.data_ptr() or None,
+          _check_like("residual", residual, device, dtype, shape),
+          _check_optional("post_weight", post_weight, device, f32, (cols,)),
+          _check_optional("gate", gate, device, f32, (cols,)),
+          _check_like("pre_weight", pre_weight, device, f32, (cols,)),
+          _check_like("residual_out", residual_out, device, dtype, shape), _check_like("y", y, device, dtype, shape),
+          _check_optional("post_rstd", post_rstd, device, f32, (rows,)),
+          _check_like("pre_rstd", pre_rstd, device, f32, (rows,)),
+          rows, cols, residual_scale, eps, _row_dtype(block), _options(cluster_size, opts))
 
 
 def residual_norm_backward_workspace_bytes(rows: int, cols: int, dtype: torch.dtype, cluster_size: int = 0,
@@ -263,39 +283,38 @@ def launch_residual_norm_backward(inputs, outputs, cluster_size: int = 0, opts=N
     dy, dresidual_out, block, residual_out, post_weight, gate, pre_weight, post_rstd, pre_rstd = inputs
     dblock, dresidual, dpost_weight, dgate, dpre_weight = outputs
     _check_matrix("dy", dy)
-    rows, cols = dy.shape
-    for name, t in (("dresidual_out", dresidual_out), ("block", block), ("residual_out", residual_out),
-                    ("dblock", dblock), ("dresidual", dresidual)):
-        if t is not None or name != "dresidual_out":
-            _check_like(name, t, dy, dy.dtype, (rows, cols))
+    rows, cols = shape = dy.shape
+    device, dtype, f32 = dy.device, dy.dtype, torch.float32
     for name, t, d in (("post_weight", post_weight, dpost_weight), ("gate", gate, dgate),
                        ("pre_weight", pre_weight, dpre_weight)):
         if (t is None) != (d is None):
             raise ValueError(f"{name} and d{name} go together")
-        if t is not None or name == "pre_weight":
-            _check_like(name, t, dy, torch.float32, (cols,))
-            _check_like(f"d{name}", d, dy, torch.float32, (cols,))
     if (post_weight is None) != (post_rstd is None):
         raise ValueError("post_weight and post_rstd go together")
-    for name, t in (("post_rstd", post_rstd), ("pre_rstd", pre_rstd)):
-        if t is not None or name == "pre_rstd":
-            _check_like(name, t, dy, torch.float32, (rows,))
-    o = _opts(cluster_size, opts)
-    with torch.cuda.device(dy.device):
-        if workspace is None:
-            need = residual_norm_backward_workspace_bytes(rows, cols, dy.dtype, 0, o)
-            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dy.device)
-        if workspace.dim() != 1:
-            raise ValueError("workspace must have one dimension")
-        _check_like("workspace", workspace, dy, torch.uint8, workspace.shape)
-        N.check(N.load().credit_residual_norm_backward(
-            _ptr(dy), _ptr(dresidual_out), _ptr(block), _ptr(residual_out), _ptr(post_weight), _ptr(gate),
-            _ptr(pre_weight), _ptr(post_rstd), _ptr(pre_rstd), _ptr(dblock), _ptr(dresidual), _ptr(dpost_weight),
-            _ptr(dgate), _ptr(dpre_weight), rows, cols, residual_scale, _row_dtype(dy), _ref(o), _ptr(workspace),
-            workspace.numel(), _stream_ptr()))
+    if workspace is None:
+        with torch.cuda.device(device):
+            need = residual_norm_backward_workspace_bytes(rows, cols, dtype, cluster_size, opts)
+        workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
+    elif workspace.dim() != 1:
+        raise ValueError("workspace must have one dimension")
+    _call(N.load().credit_residual_norm_backward, device, dy.data_ptr() or None,
+          _check_optional("dresidual_out", dresidual_out, device, dtype, shape),
+          _check_like("block", block, device, dtype, shape),
+          _check_like("residual_out", residual_out, device, dtype, shape),
+          _check_optional("post_weight", post_weight, device, f32, (cols,)),
+          _check_optional("gate", gate, device, f32, (cols,)),
+          _check_like("pre_weight", pre_weight, device, f32, (cols,)),
+          _check_optional("post_rstd", post_rstd, device, f32, (rows,)),
+          _check_like("pre_rstd", pre_rstd, device, f32, (rows,)),
+          _check_like("dblock", dblock, device, dtype, shape), _check_like("dresidual", dresidual, device, dtype, shape),
+          _check_optional("dpost_weight", dpost_weight, device, f32, (cols,)),
+          _check_optional("dgate", dgate, device, f32, (cols,)),
+          _check_like("dpre_weight", dpre_weight, device, f32, (cols,)),
+          rows, cols, residual_scale, _row_dtype(dy), _options(cluster_size, opts),
+          _check_like("workspace", workspace, device, torch.uint8, workspace.shape), workspace.numel())
 
 
-def _check_logits(name: str, t, dtype=None, shape=None) -> int:
+def _check_logits(name: str, t, device=None, dtype=None, shape=None) -> int:
     """Row stride of a [rows, cols] matrix whose rows are contiguous, whole or as the leading columns of a
     wider (padded) buffer."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -304,12 +323,15 @@ def _check_logits(name: str, t, dtype=None, shape=None) -> int:
         raise ValueError(f"{name} must have two dimensions, got {t.dim()}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
     rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+    stride, step = t.stride()
+    if (cols > 1 and step != 1) or (rows > 1 and stride < cols):
         raise ValueError(f"{name} must have contiguous rows that do not overlap")
-    return max(int(t.stride(0)), cols) if rows > 1 else cols
+    return stride if rows > 1 else cols
 
 
 def launch_token_logprobs_forward(inputs, outputs, cluster_size: int = 0, opts=None, temperature: float = 1.0) -> None:
@@ -321,28 +343,21 @@ def launch_token_logprobs_forward(inputs, outputs, cluster_size: int = 0, opts=N
     logprob, stats, entropy, top_logprob, top_index = outputs
     stride = _check_logits("logits", logits)
     rows, cols = logits.shape
+    device, f32 = logits.device, torch.float32
     if (targets is None) != (logprob is None):
         raise ValueError("targets and logprob go together")
-    if targets is not None:
-        _check_like("targets", targets, logits, torch.int64, (rows,))
-        _check_like("logprob", logprob, logits, torch.float32, (rows,))
-    _check_like("stats", stats, logits, torch.float32, (rows, 2))
-    if entropy is not None:
-        _check_like("entropy", entropy, logits, torch.float32, (rows,))
     if (top_logprob is None) != (top_index is None):
         raise ValueError("top_logprob and top_index go together")
-    top_k = 0
-    if top_index is not None:
-        if top_index.dim() != 2:
-            raise ValueError("top_index must have two dimensions")
-        top_k = int(top_index.shape[1])
-        _check_like("top_index", top_index, logits, torch.int64, (rows, top_k))
-        _check_like("top_logprob", top_logprob, logits, torch.float32, (rows, top_k))
-    o = _opts(cluster_size, opts)
-    with torch.cuda.device(logits.device):
-        N.check(N.load().credit_token_logprobs_forward(
-            _ptr(logits), stride, _ptr(targets), _ptr(logprob), _ptr(stats), _ptr(entropy), _ptr(top_logprob),
-            _ptr(top_index), top_k, rows, cols, temperature, _row_dtype(logits), _ref(o), _stream_ptr()))
+    if top_index is not None and top_index.dim() != 2:
+        raise ValueError("top_index must have two dimensions")
+    top_k = 0 if top_index is None else top_index.shape[1]
+    _call(N.load().credit_token_logprobs_forward, device, logits.data_ptr() or None, stride,
+          _check_optional("targets", targets, device, torch.int64, (rows,)),
+          _check_optional("logprob", logprob, device, f32, (rows,)), _check_like("stats", stats, device, f32, (rows, 2)),
+          _check_optional("entropy", entropy, device, f32, (rows,)),
+          _check_optional("top_logprob", top_logprob, device, f32, (rows, top_k)),
+          _check_optional("top_index", top_index, device, torch.int64, (rows, top_k)),
+          top_k, rows, cols, temperature, _row_dtype(logits), _options(cluster_size, opts))
 
 
 def launch_token_logprobs_backward(inputs, outputs, cluster_size: int = 0, opts=None, temperature: float = 1.0) -> None:
@@ -352,32 +367,24 @@ def launch_token_logprobs_backward(inputs, outputs, cluster_size: int = 0, opts=
     (dlogits,) = outputs
     stride = _check_logits("logits", logits)
     rows, cols = logits.shape
-    out_stride = _check_logits("dlogits", dlogits, logits.dtype, (rows, cols))
-    if dlogits.device != logits.device:
-        raise ValueError(f"dlogits must be on {logits.device}, got {dlogits.device}")
-    _check_like("targets", targets, logits, torch.int64, (rows,))
-    _check_like("stats", stats, logits, torch.float32, (rows, 2))
-    _check_like("dlogprob", dlogprob, logits, torch.float32, (rows,))
-    if dentropy is not None:
-        if entropy is None:
-            raise ValueError("dentropy needs the entropy of the forward pass")
-        _check_like("dentropy", dentropy, logits, torch.float32, (rows,))
-        _check_like("entropy", entropy, logits, torch.float32, (rows,))
-    o = _opts(cluster_size, opts)
-    with torch.cuda.device(logits.device):
-        N.check(N.load().credit_token_logprobs_backward(
-            _ptr(logits), stride, _ptr(targets), _ptr(stats), None if dentropy is None else _ptr(entropy),
-            _ptr(dlogprob), _ptr(dentropy), _ptr(dlogits), out_stride, rows, cols, temperature, _row_dtype(logits),
-            _ref(o), _stream_ptr()))
+    device, f32 = logits.device, torch.float32
+    out_stride = _check_logits("dlogits", dlogits, device, logits.dtype, logits.shape)
+    if dentropy is None:
+        entropy = None
+    elif entropy is None:
+        raise ValueError("dentropy needs the entropy of the forward pass")
+    _call(N.load().credit_token_logprobs_backward, device, logits.data_ptr() or None, stride,
+          _check_like("targets", targets, device, torch.int64, (rows,)),
+          _check_like("stats", stats, device, f32, (rows, 2)), _check_optional("entropy", entropy, device, f32, (rows,)),
+          _check_like("dlogprob", dlogprob, device, f32, (rows,)),
+          _check_optional("dentropy", dentropy, device, f32, (rows,)), dlogits.data_ptr() or None, out_stride, rows, cols,
+          temperature, _row_dtype(logits), _options(cluster_size, opts))
 
 
-def _check_teacher(index, value, logits) -> int:
+def _teacher_size(index) -> int:
     if not isinstance(index, torch.Tensor) or index.dim() != 2:
         raise ValueError("teacher_index must be a tensor of two dimensions")
-    top_k = int(index.shape[1])
-    _check_like("teacher_index", index, logits, torch.int64, (logits.shape[0], top_k))
-    _check_like("teacher_logprob", value, logits, torch.float32, (logits.shape[0], top_k))
-    return top_k
+    return index.shape[1]
 
 
 def launch_distill_topk_forward(inputs, outputs, cluster_size: int = 0, opts=None, temperature: float = 1.0,
@@ -390,14 +397,13 @@ def launch_distill_topk_forward(inputs, outputs, cluster_size: int = 0, opts=Non
     loss, stats = outputs
     stride = _check_logits("logits", logits)
     rows, cols = logits.shape
-    top_k = _check_teacher(index, value, logits)
-    _check_like("loss", loss, logits, torch.float32, (rows,))
-    _check_like("stats", stats, logits, torch.float32, (rows, 6))
-    o = _opts(cluster_size, opts)
-    with torch.cuda.device(logits.device):
-        N.check(N.load().credit_distill_topk_forward(
-            _ptr(logits), stride, _ptr(index), _ptr(value), top_k, _ptr(loss), _ptr(stats), rows, cols, temperature,
-            1 if tail else 0, _row_dtype(logits), _ref(o), _stream_ptr()))
+    device, f32 = logits.device, torch.float32
+    top_k = _teacher_size(index)
+    _call(N.load().credit_distill_topk_forward, device, logits.data_ptr() or None, stride,
+          _check_like("teacher_index", index, device, torch.int64, (rows, top_k)),
+          _check_like("teacher_logprob", value, device, f32, (rows, top_k)), top_k,
+          _check_like("loss", loss, device, f32, (rows,)), _check_like("stats", stats, device, f32, (rows, 6)),
+          rows, cols, temperature, 1 if tail else 0, _row_dtype(logits), _options(cluster_size, opts))
 
 
 def launch_distill_topk_backward(inputs, outputs, cluster_size: int = 0, opts=None, temperature: float = 1.0,
@@ -409,17 +415,15 @@ def launch_distill_topk_backward(inputs, outputs, cluster_size: int = 0, opts=No
     (dlogits,) = outputs
     stride = _check_logits("logits", logits)
     rows, cols = logits.shape
-    out_stride = _check_logits("dlogits", dlogits, logits.dtype, (rows, cols))
-    if dlogits.device != logits.device:
-        raise ValueError(f"dlogits must be on {logits.device}, got {dlogits.device}")
-    top_k = _check_teacher(index, value, logits)
-    _check_like("stats", stats, logits, torch.float32, (rows, 6))
-    _check_like("dloss", dloss, logits, torch.float32, (rows,))
-    o = _opts(cluster_size, opts)
-    with torch.cuda.device(logits.device):
-        N.check(N.load().credit_distill_topk_backward(
-            _ptr(logits), stride, _ptr(index), _ptr(value), top_k, _ptr(stats), _ptr(dloss), _ptr(dlogits), out_stride,
-            rows, cols, temperature, _row_dtype(logits), _ref(o), _stream_ptr()))
+    device, f32 = logits.device, torch.float32
+    out_stride = _check_logits("dlogits", dlogits, device, logits.dtype, logits.shape)
+    top_k = _teacher_size(index)
+    _call(N.load().credit_distill_topk_backward, device, logits.data_ptr() or None, stride,
+          _check_like("teacher_index", index, device, torch.int64, (rows, top_k)),
+          _check_like("teacher_logprob", value, device, f32, (rows, top_k)), top_k,
+          _check_like("stats", stats, device, f32, (rows, 6)), _check_like("dloss", dloss, device, f32, (rows,)),
+          dlogits.data_ptr() or None, out_stride, rows, cols, temperature, _row_dtype(logits),
+          _options(cluster_size, opts))
 
 
 # name -> (workload id, staged inputs, per-row input?, row-major outputs, per-row output?)
