@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "device_context.h"
 #include "vocab_rows.cuh"
@@ -19,11 +20,15 @@
 namespace credit {
 namespace {
 
-// A persistent cluster walks rows cluster, cluster + clusters, ... Its CTAs own fixed columns, 16 a thread, whose
-// parameters (and, in the backward pass, sums over the rows) stay in registers. The rows come through a ring of
-// shared-memory stages filled by bulk copies, so the next rows are on their way while one is reduced.
-constexpr int kElems = 16;      // a thread's columns
+// A persistent cluster walks rows cluster, cluster + clusters, ... Its CTAs own fixed columns, 32 bytes' worth a
+// thread, whose parameters (and, in the backward pass, sums over the rows) stay in registers. The rows come
+// through a ring of shared-memory stages filled by bulk copies, so the next rows are on their way while one is
+// reduced. A row step has one barrier: the partial sums that later steps wait for (of this row and of the next)
+// go out together, and the output of a row whose totals are known is written while they travel.
 constexpr int kMaxRing = 8;
+
+template <typename T>
+constexpr int kThreadElems = 32 / sizeof(T);   // a thread's columns
 
 struct RingArgs {
     int rows;
@@ -33,55 +38,67 @@ struct RingArgs {
     int stages;
 };
 
-// How one input's slice of a row lies: its aligned body is copied into the slot, at the place that has the
-// same alignment; elements before and behind it are read from global memory.
+// How one input's slice of a row lies: it is copied into its slot in whole 16-byte pieces, at the place that has
+// the same alignment, with what else those pieces hold. Only where a piece would reach over the matrix's first or
+// last byte is it left out; the few elements of it are then patched in (the first and last row).
 template <typename T>
 struct SliceSource {
     const T* row;   // first element of the slice in this row
     int shift;      // its distance from a 16-byte boundary, in elements
-    int head, body_end;
+    int head, body_end;   // elements [head, body_end) come with the copy
+    uint32_t bytes;       // of the copy
+    int from;             // its first element (-shift, or head)
 
-    __device__ __forceinline__ SliceSource(const void* base, int64_t offset, int local) {
+    __device__ __forceinline__ SliceSource(const void* base, int64_t offset, int local, int64_t matrix) {
         constexpr int E = 16 / sizeof(T);
         row = static_cast<const T*>(base) + offset;
         shift = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
-        head = shift == 0 ? 0 : min(E - shift, local);
-        body_end = head + (local - head) / E * E;
+        const int behind = (E - (shift + local) % E) % E;   // to the next boundary
+        const bool first = offset >= shift, last = offset + local + behind <= matrix;
+        head = first || shift == 0 ? 0 : min(E - shift, local);
+        body_end = last ? local : max(head, local - (E - behind) % E);
+        from = first ? -shift : head;
+        const int to = last ? local + behind : body_end;
+        bytes = body_end > head ? static_cast<uint32_t>(to - from) * sizeof(T) : 0;
+        if (bytes == 0) body_end = head;
     }
-    __device__ __forceinline__ uint32_t body_bytes() const { return static_cast<uint32_t>(body_end - head) * sizeof(T); }
-    __device__ __forceinline__ float element(const unsigned char* slot, int e) const {
-        return e >= head && e < body_end ? Vec<T>::load(reinterpret_cast<const T*>(slot) + shift + e) : Vec<T>::load(row + e);
+    __device__ __forceinline__ const T* place(const unsigned char* slot) const { return reinterpret_cast<const T*>(slot) + shift; }
+    __device__ __forceinline__ bool complete(int local) const { return head == 0 && body_end == local; }
+    // by all threads, when incomplete: the elements that the copy left out
+    __device__ __forceinline__ void patch(unsigned char* slot, int local) const {
+        T* at = reinterpret_cast<T*>(slot) + shift;
+        for (int e = threadIdx.x; e < head; e += blockDim.x) at[e] = row[e];
+        for (int e = body_end + threadIdx.x; e < local; e += blockDim.x) at[e] = row[e];
     }
 };
 
-// By one thread: the IN slices of `row` into `stage` (a NULL input is left out).
+// By one warp: the IN slices of a row into `stage` (a NULL input is left out), one bulk copy each: the
+// same bytes in pieces of 8 KiB or 1 KiB cost 12 % or 50 % more time at 16384 x 8192 bf16.
 template <typename T, int IN>
 __device__ __forceinline__ void fill_stage(const void* const (&in)[IN], unsigned char* stage, uint64_t* full, int64_t offset,
-                                           int local, int slot_bytes) {
-    uint32_t total = 0;
-    fence_proxy_async_smem();
+                                           int local, int64_t matrix, int slot_bytes) {
+    const int lane = threadIdx.x & 31, which = lane % IN;
+    const void* mine = in[0];
 #pragma unroll
-    for (int i = 0; i < IN; ++i)
-        if (in[i] != nullptr) total += SliceSource<T>(in[i], offset, local).body_bytes();
+    for (int i = 1; i < IN; ++i)
+        if (which == i) mine = in[i];
+    const SliceSource<T> s(mine, offset, local, matrix);
+    const uint32_t bytes = mine != nullptr ? s.bytes : 0;
+    const uint32_t total = __reduce_add_sync(0xffffffffu, lane < IN ? bytes : 0u);
     const uint32_t bar = smem_u32(full);
-    mbar_arrive_expect_tx(bar, total);
-#pragma unroll
-    for (int i = 0; i < IN; ++i) {
-        if (in[i] == nullptr) continue;
-        const SliceSource<T> s(in[i], offset, local);
-        const uint32_t bytes = s.body_bytes();
-        if (bytes != 0)
-            bulk_load_chunked(smem_u32(stage + i * slot_bytes) + (s.shift + s.head) * sizeof(T), s.row + s.head, bytes, bar);
-    }
+    if (lane == 0) mbar_arrive_expect_tx(bar, total);
+    __syncwarp();
+    if (lane < IN && bytes != 0)
+        bulk_load(smem_u32(stage + which * slot_bytes) + (s.shift + s.from) * sizeof(T), s.row + s.from, bytes, bar);
 }
 
-// W consecutive columns of one input (zeros for an input that is absent).
+// W consecutive columns of one input.
 template <typename T, int W>
-__device__ __forceinline__ void slot_elems(const unsigned char* slot, const SliceSource<T>& s, int e, float (&x)[W]) {
+__device__ __forceinline__ void slot_elems(const T* at, float (&x)[W]) {
     if constexpr (W == 1) {
-        x[0] = s.element(slot, e);
+        x[0] = Vec<T>::load(at);
     } else {
-        Vec<T>::unpack(*reinterpret_cast<const uint4*>(slot + e * sizeof(T)), x);
+        Vec<T>::unpack(*reinterpret_cast<const uint4*>(at), x);
     }
 }
 
@@ -118,70 +135,146 @@ __device__ __forceinline__ void load_channel_scale(const float* post_weight, con
     }
 }
 
-// Sums of K = 1 or 4 partials over the CTA and the cluster, in every thread, added in a fixed order. One CTA
-// barrier, and one cluster barrier when there is more than one CTA.
+// Sums of K = 2 or 4 partials over the CTA and the cluster, in every thread, added in a fixed order, in two
+// halves: publish (one CTA barrier; in a cluster every CTA then sends its sums to every other, counted on the
+// receiver's mbarrier) and collect. Two buffers: a step's publish may overtake a slow thread's collect of the step
+// before, not of the one before that.
 template <int K, int THREADS>
 struct alignas(16) RowSums {
-    float warp[THREADS / 32][K];
-    float peer[kMaxClusterSize][K];
+    float warp[2][THREADS / 32][K];
+    float peer[2][kMaxClusterSize][K];
+    uint64_t arrived[2];
 };
 
-template <int THREADS>
-__device__ __forceinline__ void row_sums(float (&v)[1], RowSums<1, THREADS>& s, uint32_t rank, uint32_t nranks) {
-    constexpr int kWarps = THREADS / 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    v[0] = warp_sum(v[0]);
-    if (lane == 0) s.warp[warp][0] = v[0];
-    __syncthreads();
-    v[0] = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) v[0] += s.warp[w][0];
-    if (nranks == 1) return;
-    if (warp == 0 && lane < static_cast<int>(nranks))
-        st_cluster_f32(map_to_rank(smem_u32(&s.peer[rank][0]), static_cast<uint32_t>(lane)), v[0]);
-    cluster_sync_all();
-    v[0] = 0.0f;
-    for (uint32_t r = 0; r < nranks; ++r) v[0] += s.peer[r][0];
+template <int K>
+struct SumsOf { using Packed = float4; };
+template <>
+struct SumsOf<2> { using Packed = float2; };
+
+__device__ __forceinline__ void add_to(float2& a, const float2& b) { a.x += b.x; a.y += b.y; }
+__device__ __forceinline__ void add_to(float4& a, const float4& b) { a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
+
+// Half the lanes go on with one of two values, the other half with the other.
+__device__ __forceinline__ float fold(float a, float b, int distance) {
+    const bool second = threadIdx.x & distance;
+    return (second ? b : a) + __shfl_xor_sync(0xffffffffu, second ? a : b, distance);
 }
 
-template <int THREADS>
-__device__ __forceinline__ void row_sums(float (&v)[4], RowSums<4, THREADS>& s, uint32_t rank, uint32_t nranks) {
-    constexpr int kWarps = THREADS / 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // four sums over 32 lanes in six shuffles: each step halves what a lane still adds up
-    const bool upper = lane & 16, odd = lane & 8;
-    float a = upper ? v[2] : v[0], b = upper ? v[3] : v[1];
-    a += __shfl_xor_sync(0xffffffffu, upper ? v[0] : v[2], 16);
-    b += __shfl_xor_sync(0xffffffffu, upper ? v[1] : v[3], 16);
-    float c = odd ? b : a;
-    c += __shfl_xor_sync(0xffffffffu, odd ? a : b, 8);
+template <int K, int THREADS>
+__device__ __forceinline__ typename SumsOf<K>::Packed cta_sums(const RowSums<K, THREADS>& s, int buf) {
+    typename SumsOf<K>::Packed t{};
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-    if ((lane & 7) == 0) s.warp[warp][lane >> 3] = c;
-    __syncthreads();
-    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        const float4 p = *reinterpret_cast<const float4*>(s.warp[w]);
-        t.x += p.x; t.y += p.y; t.z += p.z; t.w += p.w;
-    }
-    if (nranks > 1) {
-        if (warp == 0 && lane < static_cast<int>(nranks)) {
-            const uint32_t to = map_to_rank(smem_u32(&s.peer[rank][0]), static_cast<uint32_t>(lane));
-            st_cluster_f32(to, t.x);
-            st_cluster_f32(to + 4, t.y);
-            st_cluster_f32(to + 8, t.z);
-            st_cluster_f32(to + 12, t.w);
-        }
-        cluster_sync_all();
-        t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t r = 0; r < nranks; ++r) {
-            const float4 p = *reinterpret_cast<const float4*>(s.peer[r]);
-            t.x += p.x; t.y += p.y; t.z += p.z; t.w += p.w;
-        }
-    }
-    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+    for (int w = 0; w < THREADS / 32; ++w) add_to(t, *reinterpret_cast<const typename SumsOf<K>::Packed*>(s.warp[buf][w]));
+    return t;
 }
+
+template <int K, int THREADS>
+__device__ __forceinline__ void publish_sums(const float (&v)[K], RowSums<K, THREADS>& s, int buf, uint32_t rank,
+                                             uint32_t nranks) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float t;
+    if constexpr (K == 4) {
+        t = fold(fold(v[0], v[2], 16), fold(v[1], v[3], 16), 8);
+    } else {
+        t = fold(v[0], v[1], 16);
+        t += __shfl_xor_sync(0xffffffffu, t, 8);
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if ((lane & (K == 4 ? 7 : 15)) == 0) s.warp[buf][warp][lane / (32 / K)] = t;
+    __syncthreads();
+    if (nranks > 1 && warp == 0) {
+        const uint32_t bar = smem_u32(&s.arrived[buf]);
+        if (lane == 0) mbar_arrive_expect_tx(bar, nranks * K * 4);
+        const auto p = cta_sums<K, THREADS>(s, buf);
+        if (lane < static_cast<int>(nranks)) {
+            const uint32_t to = map_to_rank(smem_u32(s.peer[buf][rank]), lane), to_bar = map_to_rank(bar, lane);
+            if constexpr (K == 4) {
+                st_async_f32x4(to, p.x, p.y, p.z, p.w, to_bar);
+            } else {
+                st_async_f32x2(to, p.x, p.y, to_bar);
+            }
+        }
+    }
+}
+
+template <int K, int THREADS>
+__device__ __forceinline__ typename SumsOf<K>::Packed collect_sums(RowSums<K, THREADS>& s, int buf, uint32_t parity,
+                                                                   uint32_t nranks, int* status) {
+    if (nranks == 1) return cta_sums<K, THREADS>(s, buf);
+    mbar_wait_bounded(smem_u32(&s.arrived[buf]), parity, status);
+    typename SumsOf<K>::Packed t{};
+    for (uint32_t r = 0; r < nranks; ++r) add_to(t, *reinterpret_cast<const typename SumsOf<K>::Packed*>(s.peer[buf][r]));
+    return t;
+}
+
+// What both directions set up: this CTA's place, its ring and its barriers.
+template <typename T, int IN>
+struct RowWalk {
+    const RingArgs& a;
+    uint32_t rank, nranks;
+    int cluster, clusters;
+    int start, local;
+    int steps;               // rows of this cluster
+    int64_t matrix;          // elements
+    unsigned char* ring;
+    uint64_t* full;
+
+    __device__ __forceinline__ RowWalk(const RingArgs& args, unsigned char* ring_, uint64_t* full_) : a(args), ring(ring_), full(full_) {
+        rank = cluster_cta_rank();
+        nranks = cluster_cta_count();
+        cluster = static_cast<int>(blockIdx.x / nranks);
+        clusters = static_cast<int>(gridDim.x / nranks);
+        start = static_cast<int>(rank) * a.slice;
+        local = max(0, min(a.slice, a.cols - start));
+        steps = (a.rows - cluster + clusters - 1) / clusters;
+        matrix = static_cast<int64_t>(a.rows) * a.cols;
+    }
+    __device__ __forceinline__ int64_t row(int step) const { return cluster + static_cast<int64_t>(step) * clusters; }
+    __device__ __forceinline__ int64_t offset(int step) const { return row(step) * a.cols + start; }
+    __device__ __forceinline__ unsigned char* stage(int i) const { return ring + i * (IN * a.slot_bytes); }
+    __device__ __forceinline__ SliceSource<T> source(const void* in, int step) const { return {in, offset(step), local, matrix}; }
+    // Waits for a row's stage; PATCH: rows may be unaligned. All threads. places[k]: the slice of input k.
+    template <bool PATCH>
+    __device__ __forceinline__ void wait(const void* const (&in)[IN], const RingCursor& at, int step, const T* (&places)[IN],
+                                         int* status) const {
+        mbar_wait_bounded(smem_u32(&full[at.stage]), at.parity, status);
+#pragma unroll
+        for (int k = 0; k < IN; ++k) places[k] = reinterpret_cast<const T*>(stage(at.stage) + k * a.slot_bytes);
+        if (PATCH) {
+            bool patched = false;
+#pragma unroll
+            for (int k = 0; k < IN; ++k) {
+                if (in[k] == nullptr) continue;
+                const SliceSource<T> s = source(in[k], step);
+                places[k] += s.shift;
+                if (!s.complete(local)) {
+                    s.patch(stage(at.stage) + k * a.slot_bytes, local);
+                    patched = true;
+                }
+            }
+            if (patched) {   // the same in every thread
+                fence_proxy_async_smem();   // a later copy into this stage follows these stores
+                __syncthreads();
+            }
+        }
+    }
+    // by warp 0
+    __device__ __forceinline__ void fill(const void* const (&in)[IN], int i, int step) const {
+        if (step < steps) fill_stage<T, IN>(in, stage(i), &full[i], offset(step), local, matrix, a.slot_bytes);
+    }
+    __device__ __forceinline__ void init(const void* const (&in)[IN], uint64_t (&arrived)[2]) const {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < a.stages; ++i) mbar_init(smem_u32(&full[i]), 1);
+            mbar_init(smem_u32(&arrived[0]), 1);
+            mbar_init(smem_u32(&arrived[1]), 1);
+            fence_mbar_init();
+        }
+        __syncwarp();
+        if (threadIdx.x < 32)
+            for (int i = 0; i < a.stages; ++i) fill(in, i, i);
+    }
+};
 
 struct NormFwdArgs {
     RingArgs ring;
@@ -200,109 +293,114 @@ struct NormFwdArgs {
 };
 
 // ---------------------------------------------------------------------------
-// forward
+// forward: step i joins row i, squares row i + 1's block and writes row i - 1's y
 // ---------------------------------------------------------------------------
 template <typename T, int W, int THREADS, bool POST>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_kernel(const NormFwdArgs a) {
-    constexpr int N = kElems / W, kStride = THREADS * W;
+    constexpr int N = kThreadElems<T> / W, kStride = THREADS * W;
     __shared__ uint64_t full[kMaxRing];
-    // two reductions a row, alternating rows: a slow thread may still read the last row's
-    __shared__ RowSums<1, THREADS> sums[2][2];
+    __shared__ RowSums<2, THREADS> sums;
     extern __shared__ __align__(128) unsigned char ring[];
-    const uint32_t rank = cluster_cta_rank(), nranks = cluster_cta_count();
-    const int cluster = static_cast<int>(blockIdx.x / nranks), clusters = static_cast<int>(gridDim.x / nranks);
-    const int start = static_cast<int>(rank) * a.ring.slice;
-    const int local = max(0, min(a.ring.slice, a.ring.cols - start));
-    const int stage_bytes = 2 * a.ring.slot_bytes;
+    const RowWalk<T, 2> walk(a.ring, ring, full);
     const void* in[2] = {a.block, a.residual};
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < a.ring.stages; ++i) mbar_init(smem_u32(&full[i]), 1);
-        fence_mbar_init();
-        for (int i = 0; i < a.ring.stages; ++i) {
-            const int64_t row = cluster + static_cast<int64_t>(i) * clusters;
-            if (row < a.ring.rows)
-                fill_stage<T, 2>(in, ring + i * stage_bytes, &full[i], row * a.ring.cols + start, local, a.ring.slot_bytes);
-        }
-    }
+    walk.init(in, sums.arrived);
+    const int local = walk.local, e0 = static_cast<int>(threadIdx.x) * W;
     float c[N][W], w[N][W];
-    const int e0 = static_cast<int>(threadIdx.x) * W;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int e = e0 + u * kStride;
 #pragma unroll
         for (int j = 0; j < W; ++j) c[u][j] = w[u][j] = 0.0f;
         if (e < local) {
-            load_channel_scale<W>(a.post_weight, a.gate, start + e, c[u]);
-            load_params<W>(a.pre_weight + start + e, w[u]);
+            load_channel_scale<W>(a.post_weight, a.gate, walk.start + e, c[u]);
+            load_params<W>(a.pre_weight + walk.start + e, w[u]);
         }
     }
     __syncthreads();
-    if (nranks > 1) cluster_sync_all();
+    if (walk.nranks > 1) cluster_sync_all();
 
     const float inv_n = 1.0f / static_cast<float>(a.ring.cols);
-    RingCursor at{0, 0};
-    int turn = 0;
-    for (int64_t row = cluster; row < a.ring.rows; row += clusters, turn ^= 1) {
-        const int64_t offset = row * a.ring.cols + start;
-        unsigned char* stage = ring + at.stage * stage_bytes;
-        const SliceSource<T> os(a.block, offset, local), hs(a.residual, offset, local);
-        mbar_wait_bounded(smem_u32(&full[at.stage]), at.parity, a.status);
-        float o[N][W], h[N][W], q[1] = {0.0f};
+    RingCursor at{0, 0}, next{0, 0};
+    // sum of squares of a step's block
+    const T* ahead[2];
+    auto squares = [&](int step) {
+        float q = 0.0f;
+        walk.template wait<W == 1>(in, next, step, ahead, a.status);
+        if (POST) {
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                const int e = e0 + u * kStride;
+                if (e < local) {
+                    float o[W];
+                    slot_elems<T, W>(ahead[0] + e, o);
+#pragma unroll
+                    for (int j = 0; j < W; ++j) q = fmaf(o[j], o[j], q);
+                }
+            }
+        }
+        next.advance(a.ring.stages);
+        return q;
+    };
+    float before[N][W];   // the joined row of the step before
+    auto write_y = [&](int step, float square_sum) {
+        const float r2 = rsqrtf(fmaf(square_sum, inv_n, a.eps));
+        T* y = static_cast<T*>(a.y) + walk.offset(step);
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int e = e0 + u * kStride;
 #pragma unroll
-            for (int j = 0; j < W; ++j) o[u][j] = h[u][j] = 0.0f;
+            for (int j = 0; j < W; ++j) before[u][j] *= r2 * w[u][j];
+            if (e < local) store_elems<T, W>(y + e, before[u]);
+        }
+        if (walk.rank == 0 && threadIdx.x == 0) a.pre_rstd[walk.row(step)] = r2;
+    };
+    {
+        const float first[2] = {0.0f, squares(0)};
+        publish_sums(first, sums, 0, walk.rank, walk.nranks);
+    }
+    for (int i = 0; i < walk.steps; ++i) {
+        const float2 total = collect_sums(sums, i & 1, (i >> 1) & 1, walk.nranks, a.status);
+        const float r1 = POST ? rsqrtf(fmaf(total.y, inv_n, a.eps)) : 1.0f;
+        const int64_t offset = walk.offset(i);
+        const T *block = ahead[0], *residual = ahead[1];
+        T* out = static_cast<T*>(a.residual_out) + offset;
+        float h[N][W], part[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int e = e0 + u * kStride;
+            float o[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) o[j] = h[u][j] = 0.0f;
             if (e < local) {
-                slot_elems<T, W>(stage, os, e, o[u]);
-                slot_elems<T, W>(stage + a.ring.slot_bytes, hs, e, h[u]);
+                slot_elems<T, W>(block + e, o);
+                slot_elems<T, W>(residual + e, h[u]);
             }
 #pragma unroll
-            for (int j = 0; j < W; ++j) q[0] = fmaf(o[u][j], o[u][j], q[0]);
-        }
-        float r1 = 1.0f;
-        if (POST) {
-            row_sums(q, sums[turn][0], rank, nranks);
-            r1 = rsqrtf(fmaf(q[0], inv_n, a.eps));
-        }
-        q[0] = 0.0f;
-        T* out = static_cast<T*>(a.residual_out) + offset;
-#pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int e = e0 + u * kStride;
-#pragma unroll
             for (int j = 0; j < W; ++j) {
-                h[u][j] = fmaf(a.alpha, h[u][j], o[u][j] * r1 * c[u][j]);
-                q[0] = fmaf(h[u][j], h[u][j], q[0]);
+                h[u][j] = fmaf(a.alpha, h[u][j], o[j] * r1 * c[u][j]);
+                part[0] = fmaf(h[u][j], h[u][j], part[0]);
             }
             // stored rounded to the rows' type; y continues from the unrounded sum
             if (e < local) store_elems<T, W>(out + e, h[u]);
         }
-        row_sums(q, sums[turn][1], rank, nranks);
-        // every thread has read this stage: refill it
-        const int64_t ahead = row + static_cast<int64_t>(a.ring.stages) * clusters;
-        if (threadIdx.x == 0 && ahead < a.ring.rows)
-            fill_stage<T, 2>(in, stage, &full[at.stage], ahead * a.ring.cols + start, local, a.ring.slot_bytes);
+        if (POST && walk.rank == 0 && threadIdx.x == 0) a.post_rstd[walk.row(i)] = r1;
+        if (i + 1 < walk.steps) part[1] = squares(i + 1);
+        publish_sums(part, sums, (i + 1) & 1, walk.rank, walk.nranks);
+        if (threadIdx.x < 32) walk.fill(in, at.stage, i + a.ring.stages);   // everyone has read this stage
         at.advance(a.ring.stages);
-        const float r2 = rsqrtf(fmaf(q[0], inv_n, a.eps));
-        T* y = static_cast<T*>(a.y) + offset;
+        if (i > 0) write_y(i - 1, total.x);
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
-            const int e = e0 + u * kStride;
+        for (int u = 0; u < N; ++u)
 #pragma unroll
-            for (int j = 0; j < W; ++j) h[u][j] *= r2 * w[u][j];
-            if (e < local) store_elems<T, W>(y + e, h[u]);
-        }
-        if (rank == 0 && threadIdx.x == 0) {
-            if (POST) a.post_rstd[row] = r1;
-            a.pre_rstd[row] = r2;
-        }
+            for (int j = 0; j < W; ++j) before[u][j] = h[u][j];
     }
-    if (nranks > 1) cluster_sync_all();   // no CTA leaves while a peer may still write its sums
+    const float2 total = collect_sums(sums, walk.steps & 1, (walk.steps >> 1) & 1, walk.nranks, a.status);
+    write_y(walk.steps - 1, total.x);
+    if (walk.nranks > 1) cluster_sync_all();   // no CTA leaves while a peer may still send to it
 }
 
 // ---------------------------------------------------------------------------
-// backward
+// backward: step i takes row i + 1's sums and writes row i's gradients
 // ---------------------------------------------------------------------------
 struct NormBwdArgs {
     RingArgs ring;
@@ -327,105 +425,124 @@ struct NormBwdArgs {
 // so its three sums travel with sum t v. Both passes over a row read it from its stage.
 template <typename T, int W, int THREADS, bool POST>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_bwd_kernel(const NormBwdArgs a) {
-    constexpr int N = kElems / W, kStride = THREADS * W;
+    constexpr int N = kThreadElems<T> / W, kStride = THREADS * W;
     __shared__ uint64_t full[kMaxRing];
-    __shared__ RowSums<4, THREADS> sums[2];   // alternating rows: a slow thread may still read the other
+    __shared__ RowSums<4, THREADS> sums;
     extern __shared__ __align__(128) unsigned char ring[];
-    const uint32_t rank = cluster_cta_rank(), nranks = cluster_cta_count();
-    const int cluster = static_cast<int>(blockIdx.x / nranks), clusters = static_cast<int>(gridDim.x / nranks);
-    const int start = static_cast<int>(rank) * a.ring.slice;
-    const int local = max(0, min(a.ring.slice, a.ring.cols - start));
-    const int slot = a.ring.slot_bytes, stage_bytes = 4 * slot;
+    const RowWalk<T, 4> walk(a.ring, ring, full);
     const void* in[4] = {a.dy, a.block, a.residual_out, a.dresidual_out};
+    walk.init(in, sums.arrived);
+    const int local = walk.local, e0 = static_cast<int>(threadIdx.x) * W;
     const bool has_d = a.dresidual_out != nullptr;
-    auto fill = [&](int i, int64_t row) {
-        fill_stage<T, 4>(in, ring + i * stage_bytes, &full[i], row * a.ring.cols + start, local, slot);
-    };
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < a.ring.stages; ++i) mbar_init(smem_u32(&full[i]), 1);
-        fence_mbar_init();
-        for (int i = 0; i < a.ring.stages; ++i) {
-            const int64_t row = cluster + static_cast<int64_t>(i) * clusters;
-            if (row < a.ring.rows) fill(i, row);
-        }
-    }
     float c[N][W], w[N][W], col_c[N][W], col_w[N][W];
-    const int e0 = static_cast<int>(threadIdx.x) * W;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int e = e0 + u * kStride;
 #pragma unroll
         for (int j = 0; j < W; ++j) c[u][j] = w[u][j] = col_c[u][j] = col_w[u][j] = 0.0f;
         if (e < local) {
-            load_channel_scale<W>(a.post_weight, a.gate, start + e, c[u]);
-            load_params<W>(a.pre_weight + start + e, w[u]);
+            load_channel_scale<W>(a.post_weight, a.gate, walk.start + e, c[u]);
+            load_params<W>(a.pre_weight + walk.start + e, w[u]);
         }
     }
+    // the rows' rstd: cold lines, fetched a step ahead of their first use
+    float r1_next = POST ? a.post_rstd[walk.row(0)] : 1.0f, r2_next = a.pre_rstd[walk.row(0)];
     __syncthreads();
-    if (nranks > 1) cluster_sync_all();
+    if (walk.nranks > 1) cluster_sync_all();
 
     const float inv_n = 1.0f / static_cast<float>(a.ring.cols);
     RingCursor at{0, 0};
-    int turn = 0, last = -1;   // the stage of the row before
-    float r1_next = POST && cluster < a.ring.rows ? a.post_rstd[cluster] : 1.0f;
-    float r2_next = cluster < a.ring.rows ? a.pre_rstd[cluster] : 1.0f;
-    for (int64_t row = cluster; row < a.ring.rows; row += clusters, turn ^= 1) {
-        const int64_t offset = row * a.ring.cols + start;
-        const unsigned char* stage = ring + at.stage * stage_bytes;
-        const SliceSource<T> ys(a.dy, offset, local), os(a.block, offset, local), hs(a.residual_out, offset, local),
-            ds(has_d ? a.dresidual_out : a.dy, offset, local);
-        const float r1 = r1_next, r2 = r2_next;
-        if (row + clusters < a.ring.rows) {   // a cold line each: a row ahead
-            if (POST) r1_next = a.post_rstd[row + clusters];
-            r2_next = a.pre_rstd[row + clusters];
+    // what fits the registers between the two passes leaves the stage free for the next row
+    constexpr bool kKeep = W > 1 || sizeof(T) == 4;
+    using Raw = std::conditional_t<(W > 1), uint4, T>;
+    Raw kept[kKeep ? N : 1][4];
+    const T* places[4];
+    // W columns of the four inputs, as they are
+    auto fetch = [&](int e, Raw (&raw)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            raw[k] = Raw{};
+            if (k < 3 || has_d) raw[k] = *reinterpret_cast<const Raw*>(places[k] + e);
         }
-        mbar_wait_bounded(smem_u32(&full[at.stage]), at.parity, a.status);
-        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    auto widen = [&](const Raw& raw, float (&x)[W]) {
+        if constexpr (W > 1) {
+            Vec<T>::unpack(raw, x);
+        } else {
+            x[0] = Vec<T>::load(&raw);
+        }
+    };
+    // a row's partial sums (with the rstd that *_next hold), and its part of dpre_weight
+    auto reduce_row = [&](int step, float (&part)[4]) {
+        walk.template wait<W == 1>(in, at, step, places, a.status);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[k] = 0.0f;
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int e = e0 + u * kStride;
             if (e < local) {
+                Raw mine[4];
+                fetch(e, mine);
                 float dy[W], n[W], v[W], d[W];
-                slot_elems<T, W>(stage, ys, e, dy);
-                slot_elems<T, W>(stage + slot, os, e, n);
-                slot_elems<T, W>(stage + 2 * slot, hs, e, v);
-#pragma unroll
-                for (int j = 0; j < W; ++j) d[j] = 0.0f;
-                if (POST && has_d) slot_elems<T, W>(stage + 3 * slot, ds, e, d);
+                widen(mine[0], dy);
+                widen(mine[1], n);
+                widen(mine[2], v);
+                widen(mine[3], d);
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
-                    v[j] *= r2;
+                    v[j] *= r2_next;
                     const float t = dy[j] * w[u][j];
                     part[0] = fmaf(t, v[j], part[0]);
                     if (POST) {
-                        const float cn = c[u][j] * (n[j] * r1);
+                        const float cn = c[u][j] * (n[j] * r1_next);
                         part[1] = fmaf(cn, d[j], part[1]);
                         part[2] = fmaf(cn, t, part[2]);
                         part[3] = fmaf(cn, v[j], part[3]);
                     }
                     col_w[u][j] = fmaf(dy[j], v[j], col_w[u][j]);
                 }
+                if constexpr (kKeep) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) kept[u][k] = mine[k];
+                }
             }
         }
-        row_sums(part, sums[turn], rank, nranks);
-        // every thread is done with the row before: refill its stage
-        if (threadIdx.x == 0 && last >= 0) {
-            const int64_t ahead = row + static_cast<int64_t>(a.ring.stages - 1) * clusters;
-            if (ahead < a.ring.rows) fill(last, ahead);
+    };
+    float part[4];
+    int last = -1;   // stage of the row before
+    for (int i = 0; i < walk.steps; ++i) {
+        reduce_row(i, part);
+        publish_sums(part, sums, i & 1, walk.rank, walk.nranks);
+        if (kKeep) {   // the row is in registers
+            if (threadIdx.x < 32) walk.fill(in, at.stage, i + a.ring.stages);
+        } else if (threadIdx.x < 32 && last >= 0) {   // everyone is done with the row before
+            walk.fill(in, last, i - 1 + a.ring.stages);
         }
-        const float m1 = part[0] * inv_n;
-        const float m2 = POST ? (part[1] + r2 * (part[2] - m1 * part[3])) * inv_n : 0.0f;
+        const float r1 = r1_next, r2 = r2_next;
+        if (i + 1 < walk.steps) {
+            if (POST) r1_next = a.post_rstd[walk.row(i + 1)];
+            r2_next = a.pre_rstd[walk.row(i + 1)];
+        }
+        const float4 total = collect_sums(sums, i & 1, (i >> 1) & 1, walk.nranks, a.status);
+        const float m1 = total.x * inv_n;
+        const float m2 = POST ? (total.y + r2 * (total.z - m1 * total.w)) * inv_n : 0.0f;
+        const int64_t offset = walk.offset(i);
 #pragma unroll
         for (int u = 0; u < N; ++u) {
             const int e = e0 + u * kStride;
             if (e < local) {
-                float dy[W], n[W], v[W], d[W];
-                slot_elems<T, W>(stage, ys, e, dy);
-                slot_elems<T, W>(stage + slot, os, e, n);
-                slot_elems<T, W>(stage + 2 * slot, hs, e, v);
+                Raw mine[4];
+                if constexpr (kKeep) {
 #pragma unroll
-                for (int j = 0; j < W; ++j) d[j] = 0.0f;
-                if (has_d) slot_elems<T, W>(stage + 3 * slot, ds, e, d);
+                    for (int k = 0; k < 4; ++k) mine[k] = kept[u][k];
+                } else {
+                    fetch(e, mine);
+                }
+                float dy[W], n[W], v[W], d[W];
+                widen(mine[0], dy);
+                widen(mine[1], n);
+                widen(mine[2], v);
+                widen(mine[3], d);
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
                     n[j] *= r1;
@@ -438,15 +555,10 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_bwd_kern
                 store_elems<T, W>(static_cast<T*>(a.dresidual) + offset + e, d);
             }
         }
-        if (a.ring.stages == 1) {   // nothing to hide behind: refill at once
-            __syncthreads();
-            if (threadIdx.x == 0 && row + clusters < a.ring.rows) fill(0, row + clusters);
-        } else {
-            last = at.stage;
-        }
+        last = at.stage;
         at.advance(a.ring.stages);
     }
-    float* mine = a.partials + static_cast<size_t>(cluster) * 2 * a.ring.cols + start;
+    float* mine = a.partials + static_cast<size_t>(walk.cluster) * 2 * a.ring.cols + walk.start;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int e = e0 + u * kStride;
@@ -458,7 +570,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_bwd_kern
             }
         }
     }
-    if (nranks > 1) cluster_sync_all();   // no CTA leaves while a peer may still write its sums
+    if (walk.nranks > 1) cluster_sync_all();   // no CTA leaves while a peer may still send to it
 }
 
 // Adds the clusters' column sums in a fixed order: 32 columns a CTA, 32 strands of clusters.
@@ -530,31 +642,27 @@ struct Plan {
 
 int round_to(int64_t v, int m) { return static_cast<int>((v + m - 1) / m * m); }
 
-// The shape's part of a plan, without a device: cluster size, slice and threads. A CTA holds 8192 columns (16
-// for each of 512 threads). The automatic cluster is the smallest whose slices do, and whose stages are at most
-// 72 KiB, so that three fit an SM.
-int plan_shape(int64_t cols, int dtype, bool vector, int inputs, int asked, Plan* p, const Form** form) {
-    const int size = dtype == CREDIT_BF16 ? 2 : 4;
-    const int64_t most = 512 * kElems;
+// The shape's part of a plan, without a device: cluster size, slice and threads. A CTA holds 16 KiB of a row (32
+// bytes for each of 512 threads), so that three stages of four inputs fit an SM; the automatic cluster is the
+// smallest that holds the row.
+int plan_shape(int64_t cols, int dtype, bool vector, int asked, Plan* p, const Form** form) {
+    const int size = dtype == CREDIT_BF16 ? 2 : 4, each = 32 / size;
+    const int64_t most = 512 * each;
     int cluster = asked;
-    if (cluster == 0) {
-        for (cluster = 1; cluster < kMaxClusterSize; cluster *= 2) {
-            const int64_t slice = (cols + cluster - 1) / cluster;
-            if (slice <= most && slice * size * inputs <= 72 * 1024) break;
-        }
-    }
+    if (cluster == 0)
+        for (cluster = 1; cluster < kMaxClusterSize && (cols + cluster - 1) / cluster > most; cluster *= 2) {}
     const int64_t slice = cluster == 1 ? cols : round_to((cols + cluster - 1) / cluster, 64);
     if (slice > most)
         return report_error(CREDIT_ERR_UNSUPPORTED, "cols=%lld: a cluster of %d holds at most %lld columns of a row",
                             static_cast<long long>(cols), cluster, static_cast<long long>(most) * cluster);
     const Form* f = dtype == CREDIT_BF16 ? forms<__nv_bfloat16>(vector) : forms<float>(vector);
-    while (static_cast<int64_t>(f->threads) * kElems < slice) ++f;
+    while (static_cast<int64_t>(f->threads) * each < slice) ++f;
     *form = f;
     p->threads = f->threads;
     p->cluster = cluster;
     p->ring.cols = static_cast<int>(cols);
     p->ring.slice = static_cast<int>(slice);
-    p->ring.slot_bytes = round_to(slice * size + 16, 128);
+    p->ring.slot_bytes = round_to(slice * size + 32, 128);
     return CREDIT_OK;
 }
 
@@ -571,7 +679,7 @@ int plan_launch(int64_t rows, const void* func, int inputs, Plan* p) {
     const int room = p->ctx.max_dynamic_smem - 4096;                      // of one CTA alone
     const int share = (p->ctx.max_dynamic_smem + 1024) / per_sm - 4096;   // 1 KiB of it is the system's
     int stages = share / stage;
-    if (stages < 2) stages = room / stage < 2 ? 1 : 2;
+    if (stages < 3) stages = room / stage < 3 ? room / stage : 3;   // 16 KiB slots: never fewer than three
     stages = stages > kMaxRing ? kMaxRing : stages;
     p->ring.stages = stages;
     p->ring.rows = static_cast<int>(rows);
@@ -610,7 +718,7 @@ int forward(const void* block, const void* residual, const float* post_weight, c
                         all_aligned({block, residual, post_weight, gate, pre_weight, residual_out, y});
     const Form* form = nullptr;
     Plan p;
-    rc = plan_shape(cols, dtype, vector, 2, asked, &p, &form);
+    rc = plan_shape(cols, dtype, vector, asked, &p, &form);
     if (rc != CREDIT_OK || rows == 0) return rc;
     if (any_null({block, residual, pre_weight, residual_out, y, pre_rstd}))
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "block, residual, pre_weight, residual_out, y and pre_rstd must not be NULL");
@@ -641,7 +749,7 @@ size_t partial_bytes(const Plan& p) { return static_cast<size_t>(p.clusters) * 2
 
 int plan_backward(int64_t rows, int64_t cols, int dtype, bool vector, bool post, int asked, Plan* p) {
     const Form* form = nullptr;
-    int rc = plan_shape(cols, dtype, vector, 4, asked, p, &form);
+    int rc = plan_shape(cols, dtype, vector, asked, p, &form);
     if (rc != CREDIT_OK) return rc;
     return plan_launch(rows, form->backward[post], 4, p);
 }

@@ -299,9 +299,9 @@ int credit_layernorm_backward_stats_static(const void* x, const void* dy, const 
  * post_weight (with post_rstd) and gate may be NULL: no post norm, no gate. y is
  * computed from the unrounded sum. post_rstd and pre_rstd are fp32 [rows] outputs, what
  * the backward call needs. residual_out may be residual or block, y may be block or
- * residual, y and residual_out must differ. Rows up to 131072 columns (a row lives in the registers
- * of a cluster); a wider row, or one wider than the asked cluster holds, gives
- * CREDIT_ERR_UNSUPPORTED. Of the launch options, cluster_size only.
+ * residual, y and residual_out must differ. A CTA of the row's cluster holds 16 KiB of it: rows up to
+ * 131072 bf16 or 65536 fp32 columns; a wider row, or one wider than the asked cluster
+ * holds, gives CREDIT_ERR_UNSUPPORTED. Of the launch options, cluster_size only.
  * No reference kernel exists for this; it stands beside credit_rmsnorm_forward. */
 int credit_residual_norm_forward(const void* block, const void* residual, const float* post_weight,
                                  const float* gate, const float* pre_weight, void* residual_out, void* y,

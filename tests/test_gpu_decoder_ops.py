@@ -96,7 +96,7 @@ def _check_norm_forward(inputs, got, scale, eps, dtype):
 
 
 NORM_SHAPES = [(1, 1, 0), (3, 7, 0), (2, 64, 2), (5, 1000, 0), (4, 1024, 4), (300, 1024, 0), (3, 4099, 0), (2, 8192, 16),
-               (2, 8200, 0), (3, 16384, 0), (2, 16392, 0), (2, 33333, 8), (1, 131072, 0), (700, 72, 0)]
+               (2, 8200, 0), (3, 16384, 0), (2, 16392, 0), (2, 33333, 16), (1, 65536, 0), (700, 72, 0), (40, 9000, 0), (900, 5000, 2)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
