@@ -302,85 +302,53 @@ struct DistillBwdArgs {
     int64_t out_ld;
     int cols;
     int pieces;
+    int chunks;
     float inv_t;
     int* status;
 };
 
 template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(const DistillBwdArgs a) {
-    constexpr int E = Vec<T>::kElems;
+__global__ void __launch_bounds__(kThreads, 6) distill_topk_bwd_kernel(const DistillBwdArgs a) {
     __shared__ int column[kMaxList];
     const int64_t row = blockIdx.x / a.pieces;
     const int piece = static_cast<int>(blockIdx.x % a.pieces);
     const int tid = threadIdx.x;
-    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-    T* out = static_cast<T*>(a.dlogits) + row * a.out_ld;
+    const RowMap<T, kThreads, kUnroll, VECTOR> map(static_cast<const T*>(a.logits) + row * a.ld,
+                                                   static_cast<T*>(a.dlogits) + row * a.out_ld, a.cols, piece, a.chunks);
     const float* s = a.stats + row * kStats;
     const float all_m = s[0], all_log = s[1], tail_m = s[2], tail_log = s[3], log_norm = s[4], rest = s[5];
     const float k2 = a.inv_t * kLog2e;
     float g = a.dloss[row] * a.inv_t;
+    uint4 v[kUnroll];
+    map.first_chunk(v);
 
     // this thread's list entry: its column, the student's logit there (before anything is written: the
     // gradient may take the logits' place) and whether the column lies in this CTA's piece
     const int64_t given = tid < a.top_k ? a.index[row * a.top_k + tid] : -1;
     const bool bad = given >= a.cols;
     const int c = given < 0 || bad ? -1 : static_cast<int>(given);
-    const RowSpan<T> span(x, 0, a.cols);
-    const int v0 = piece * kThreads * kUnroll;   // first vector (or first scalar / E) of the piece
-    auto in_piece = [&](int col) {
-        if (!VECTOR) return col / (kThreads * kUnroll * E) == piece;
-        const int v = col - span.head;
-        if (v < 0 || v >= span.nvec * E) return piece == 0;
-        return v / (kThreads * kUnroll * E) == piece;
-    };
-    const bool mine = c >= 0 && in_piece(c);
-    float xl = 0.0f;
-    if (mine) xl = Vec<T>::load(x + c);
+    const bool mine = c >= 0 && map.holds(c);
+    const float listed = mine ? Vec<T>::load(map.x + c) : 0.0f;
     if (tid < kMaxList) column[tid] = c;
-    // also the barrier between the loads above and the first write; 1: some column, 2: one outside the row
-    const int seen = (c >= 0 ? 1 : 0) | (bad ? 2 : 0);
-    const int any = (__syncthreads_or(seen & 1) ? 1 : 0) | (__syncthreads_or(seen & 2) ? 2 : 0);
+    // also the barrier between the loads above and the first write
+    const bool any = __syncthreads_or(c >= 0), outside = __syncthreads_or(bad);
 
     // no teacher, or no unmasked logit: no gradient
-    const bool zero = any == 0 || all_m == -CUDART_INF_F;
-    if (any & 2) {
+    const bool zero = (!any && !outside) || all_m == -CUDART_INF_F;
+    if (outside) {
         if (piece == 0 && tid == 0) atomicOr(a.status, kStatusBadIndex);
         g = CUDART_NAN_F;
     }
     if (is_broken(all_m)) g = CUDART_NAN_F;
     // outside the list: exp(z - tail lse) * (q_r - w_r); tail_m = -inf says that every such logit is masked
-    const float factor = zero ? 0.0f : g * (ex2_approx((tail_m - all_m) * k2 + (tail_log - all_log) * kLog2e) - rest);
+    const float factor = g * (ex2_approx((tail_m - all_m) * k2 + (tail_log - all_log) * kLog2e) - rest);
     const float base = tail_m == -CUDART_INF_F ? 0.0f : tail_m, log2_sum = tail_log * kLog2e;
-    auto grad = [&](float xv) { return ex2_approx(fmaf(xv - base, k2, -log2_sum)) * factor; };
-
-    if (!VECTOR) {
-        const int first = v0 * E, last = min(a.cols, first + kThreads * kUnroll * E);
-        for (int i = first + tid; i < last; i += kThreads)
-            Vec<T>::store(out + i, zero ? 0.0f : grad(Vec<T>::load(x + i)));
-    } else {
-        const uint4* in_vec = span.vectors();
-        uint4* out_vec = reinterpret_cast<uint4*>(out + span.head);
-        if (piece == 0 && tid < span.edges) {
-            const int i = span.edge_offset(tid);
-            Vec<T>::store(out + i, zero ? 0.0f : grad(Vec<T>::load(x + i)));
-        }
-        uint4 v[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int i = v0 + tid + u * kThreads;
-            v[u] = !zero && i < span.nvec ? load_stream(in_vec + i) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int i = v0 + tid + u * kThreads;
-            if (i >= span.nvec) break;
-            float y[E];
-            Vec<T>::unpack(v[u], y);
-#pragma unroll
-            for (int j = 0; j < E; ++j) y[j] = zero ? 0.0f : grad(y[j]);
-            __stcs(out_vec + i, Vec<T>::pack(y));
-        }
-    }
+    const float2 minus = make_float2(-base, -base), scale = make_float2(k2, k2), shift = make_float2(-log2_sum, -log2_sum),
+                 by = make_float2(factor, factor);
+    map.run(zero, v, [&](float2 z) {
+        const float2 d = __ffma2_rn(__fadd2_rn(z, minus), scale, shift);
+        return __fmul2_rn(make_float2(ex2_approx(d.x), ex2_approx(d.y)), by);
+    });
     if (zero) return;
     __syncthreads();   // the piece is written; the listed columns follow
     if (mine) {
@@ -393,8 +361,8 @@ __global__ void __launch_bounds__(kThreads) distill_topk_bwd_kernel(const Distil
                 w += expf(a.teacher[row * a.top_k + k] - log_norm);
             }
         }
-        const float q = ex2_approx(fmaf(xl - all_m, k2, -all_log * kLog2e));
-        if (!earlier) Vec<T>::store(out + c, g * (q - w));
+        const float q = ex2_approx(fmaf(listed - all_m, k2, -all_log * kLog2e));
+        if (!earlier) Vec<T>::store(map.out + c, g * (q - w));
     }
 }
 
@@ -485,8 +453,9 @@ int backward(const void* logits, int64_t ld, const int64_t* index, const float* 
     a.inv_t = 1.0f / temperature;
     a.status = ctx.status;
     const bool vector = same_phase(logits, ld, dlogits, out_ld, rows, dtype);
-    const int per_piece = kThreads * kUnroll * (dtype == CREDIT_BF16 ? 8 : 4);
-    a.pieces = static_cast<int>((cols + per_piece - 1) / per_piece);
+    const int chunk = kThreads * kUnroll * (dtype == CREDIT_BF16 ? 8 : 4);
+    a.chunks = chunks_per_piece(rows, cols, chunk, 4, ctx.sm_count);   // 1, 2, 4, 8: 239, 190, 175, 184 us at 2048 x 131072 bf16
+    a.pieces = static_cast<int>((cols + static_cast<int64_t>(chunk) * a.chunks - 1) / (static_cast<int64_t>(chunk) * a.chunks));
     const void* func;
     if (dtype == CREDIT_BF16)
         func = vector ? reinterpret_cast<const void*>(&distill_topk_bwd_kernel<__nv_bfloat16, true>)

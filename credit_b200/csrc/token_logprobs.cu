@@ -177,95 +177,51 @@ struct LogprobBwdArgs {
     int64_t out_ld;
     int cols;
     int pieces;              // CTAs per row
+    int chunks;              // of a piece
     float inv_t;
     int* status;
 };
 
-struct LogprobRow {
-    float base, k2, log2_sum;   // log2 p = (x - base) * k2 - log2_sum
-    float g, gh, h2;            // upstream gradients over the temperature, entropy / ln 2
-    int target;
-};
-
-template <bool ENTROPY>
-__device__ __forceinline__ float logprob_grad(float x, const LogprobRow& r) {
-    float d = fmaf(x - r.base, r.k2, -r.log2_sum);
-    if (ENTROPY) {
-        d = fmaxf(d, -200.0f);   // p = 0 there, and 0 * -inf is kept out
-        return -ex2_approx(d) * fmaf(r.gh, d + r.h2, r.g);
-    }
-    return -ex2_approx(d) * r.g;
-}
-
 template <typename T, bool ENTROPY, bool VECTOR>
-__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const LogprobBwdArgs a) {
+__global__ void __launch_bounds__(kThreads, 6) token_logprobs_bwd_kernel(const LogprobBwdArgs a) {
     const int64_t row = blockIdx.x / a.pieces;
     const int piece = static_cast<int>(blockIdx.x % a.pieces);
-    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-    T* out = static_cast<T*>(a.dlogits) + row * a.out_ld;
+    const RowMap<T, kThreads, kUnroll, VECTOR> map(static_cast<const T*>(a.logits) + row * a.ld,
+                                                   static_cast<T*>(a.dlogits) + row * a.out_ld, a.cols, piece, a.chunks);
+    uint4 v[kUnroll];
     const int64_t target = a.targets[row];
-    LogprobRow r;
-    r.base = a.stats[2 * row];
-    r.k2 = a.inv_t * kLog2e;
-    r.log2_sum = a.stats[2 * row + 1] * kLog2e;
-    r.g = a.dlogprob[row] * a.inv_t;
-    r.gh = ENTROPY ? a.dentropy[row] * a.inv_t * kLn2 : 0.0f;
-    r.h2 = ENTROPY ? a.entropy[row] * kLog2e : 0.0f;
-    r.target = static_cast<int>(target);
+    const float base = a.stats[2 * row], k2 = a.inv_t * kLog2e, log2_sum = a.stats[2 * row + 1] * kLog2e;
+    // upstream gradients over the temperature, that of the entropy per unit of log2 p
+    float g = a.dlogprob[row] * a.inv_t;
+    const float gh = ENTROPY ? a.dentropy[row] * a.inv_t * kLn2 : 0.0f, h2 = ENTROPY ? a.entropy[row] * kLog2e : 0.0f;
     // an ignored row, or one without an unmasked logit: no gradient
-    const bool zero = target < 0 || r.base == -CUDART_INF_F;
+    const bool zero = target < 0 || base == -CUDART_INF_F;
+    if (!zero) map.first_chunk(v);
     if (target >= a.cols) {
         if (piece == 0 && threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
-        r.g = CUDART_NAN_F;
+        g = CUDART_NAN_F;
     }
-    if (is_broken(r.base)) r.g = CUDART_NAN_F;   // NaN or +inf in the row: NaN throughout
-    // at the target: + g, with 1 - p taken by expm1 so that nothing cancels when p is near 1
-    auto at_target = [&](float xv) {
-        const float d = fmaf(xv - r.base, r.k2, -r.log2_sum);
-        const float dc = fmaxf(d, -200.0f);
-        const float entropy_part = ENTROPY ? -ex2_approx(dc) * r.gh * (dc + r.h2) : 0.0f;
-        return fmaf(r.g, -expm1f(d * kLn2), entropy_part);
-    };
-    auto grad = [&](float xv, int column) {
-        if (zero) return 0.0f;
-        return column == r.target ? at_target(xv) : logprob_grad<ENTROPY>(xv, r);
-    };
-
-    if (!VECTOR) {
-        const int first = piece * kThreads * kUnroll * Vec<T>::kElems;
-        const int last = min(a.cols, first + kThreads * kUnroll * Vec<T>::kElems);
-        for (int c = first + static_cast<int>(threadIdx.x); c < last; c += kThreads)
-            Vec<T>::store(out + c, grad(zero ? 0.0f : Vec<T>::load(x + c), c));
-        return;
-    }
-    constexpr int E = Vec<T>::kElems;
-    const RowSpan<T> span(x, 0, a.cols);
-    const uint4* in_vec = span.vectors();
-    uint4* out_vec = reinterpret_cast<uint4*>(out + span.head);
-    if (piece == 0 && static_cast<int>(threadIdx.x) < span.edges) {
-        const int c = span.edge_offset(threadIdx.x);
-        Vec<T>::store(out + c, grad(zero ? 0.0f : Vec<T>::load(x + c), c));
-    }
-    const int i0 = piece * kThreads * kUnroll + static_cast<int>(threadIdx.x);
-    uint4 v[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-        v[u] = !zero && i0 + u * kThreads < span.nvec ? load_stream(in_vec + i0 + u * kThreads) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-        const int i = i0 + u * kThreads;
-        if (i >= span.nvec) break;
-        float y[E];
-        if (zero) {
-            __stcs(out_vec + i, make_uint4(0, 0, 0, 0));
-            continue;
+    if (is_broken(base)) g = CUDART_NAN_F;   // NaN or +inf in the row: NaN throughout
+    // the target's element is overwritten by the thread that writes the others around it: + g, with 1 - p taken
+    // by expm1 so that nothing cancels when p is near 1
+    const bool mine = !zero && target < a.cols && map.owns(static_cast<int>(target));
+    const float at_target = mine ? Vec<T>::load(map.x + target) : 0.0f;
+    const float2 minus = make_float2(-base, -base), scale = make_float2(k2, k2), shift = make_float2(-log2_sum, -log2_sum);
+    const float2 gh_2 = make_float2(-gh, -gh), rest = make_float2(-fmaf(gh, h2, g), -fmaf(gh, h2, g));
+    map.run(zero, v, [&](float2 z) {
+        float2 d = __ffma2_rn(__fadd2_rn(z, minus), scale, shift);   // log2 p
+        float2 weight = rest;
+        if (ENTROPY) {
+            d.x = fmaxf(d.x, -200.0f);   // p = 0 there, and 0 * -inf is kept out
+            d.y = fmaxf(d.y, -200.0f);
+            weight = __ffma2_rn(gh_2, d, rest);
         }
-        Vec<T>::unpack(v[u], y);
-        const int hit = r.target - span.vector_column(i);
-        const float picked = hit >= 0 && hit < E ? at_target(Vec<T>::load(x + r.target)) : 0.0f;
-#pragma unroll
-        for (int j = 0; j < E; ++j) y[j] = j == hit ? picked : logprob_grad<ENTROPY>(y[j], r);
-        __stcs(out_vec + i, Vec<T>::pack(y));
+        return __fmul2_rn(make_float2(ex2_approx(d.x), ex2_approx(d.y)), weight);
+    });
+    if (mine) {
+        const float d = fmaf(at_target - base, k2, -log2_sum), dc = fmaxf(d, -200.0f);
+        const float entropy_part = ENTROPY ? -ex2_approx(dc) * gh * (dc + h2) : 0.0f;
+        Vec<T>::store(map.out + target, fmaf(g, -expm1f(d * kLn2), entropy_part));
     }
 }
 
@@ -368,8 +324,9 @@ int backward(const void* logits, int64_t ld, const int64_t* targets, const float
     a.inv_t = 1.0f / temperature;
     a.status = ctx.status;
     const bool vector = same_phase(logits, ld, dlogits, out_ld, rows, dtype);
-    const int per_piece = kThreads * kUnroll * (dtype == CREDIT_BF16 ? 8 : 4);
-    a.pieces = static_cast<int>((cols + per_piece - 1) / per_piece);
+    const int chunk = kThreads * kUnroll * (dtype == CREDIT_BF16 ? 8 : 4);
+    a.chunks = chunks_per_piece(rows, cols, chunk, 2, ctx.sm_count);   // 1, 2, 4, 8: 156, 155, 163, 169 us at 4096 x 65536 bf16
+    a.pieces = static_cast<int>((cols + static_cast<int64_t>(chunk) * a.chunks - 1) / (static_cast<int64_t>(chunk) * a.chunks));
     const void* func = dtype == CREDIT_BF16 ? backward_kernel<__nv_bfloat16>(dentropy != nullptr, vector)
                                             : backward_kernel<float>(dentropy != nullptr, vector);
     rc = prepare_kernel(ctx, func);

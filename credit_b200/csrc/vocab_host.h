@@ -54,6 +54,13 @@ inline bool same_phase(const void* logits, int64_t ld, const void* dlogits, int6
     return (in - out) % 16 == 0 && (rows == 1 || (ld - out_ld) * size % 16 == 0);
 }
 
+// Chunks of a row that one CTA of an elementwise kernel takes: up to `most`, over which what a CTA does once is
+// spread, as long as that leaves 16 CTAs an SM.
+inline int chunks_per_piece(int64_t rows, int64_t cols, int chunk_elems, int most, int sm_count) {
+    const int64_t all = (cols + chunk_elems - 1) / chunk_elems, each = rows * all / (16 * sm_count);
+    return static_cast<int>(each < 1 ? 1 : (each > most ? most : each));
+}
+
 inline int row_slice(int64_t cols, int cluster) { return static_cast<int>(((cols + cluster - 1) / cluster + 63) / 64 * 64); }
 
 // CTAs per row of the kernels that reduce a row.

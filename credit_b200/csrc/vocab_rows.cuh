@@ -212,6 +212,89 @@ __device__ __forceinline__ float edge_element(const RowSpan<T>& s) {
     return i < s.edges ? Vec<T>::load(s.first + s.edge_offset(i)) : -CUDART_INF_F;
 }
 
+// Elementwise over chunks [piece * chunks, (piece + 1) * chunks) of a row (and its edges, in piece 0):
+// out = f(x) for pairs of elements, or zeros. out may be x. VECTOR: both start at the same place between two
+// 16-byte boundaries. Element c belongs to the thread that owns(c) names.
+template <typename T, int THREADS, int U, bool VECTOR>
+struct RowMap {
+    const T* x;
+    T* out;
+    RowSpan<T> span;
+    int cols, piece, chunks;
+
+    __device__ __forceinline__ RowMap(const T* x_, T* out_, int cols_, int piece_, int chunks_)
+        : x(x_), out(out_), span(x_, 0, cols_), cols(cols_), piece(piece_), chunks(chunks_) {}
+
+    static constexpr int kVecs = THREADS * U;
+    __device__ __forceinline__ int piece_elems() const { return chunks * kVecs * Vec<T>::kElems; }
+
+    // whether column c is this thread's
+    __device__ __forceinline__ bool owns(int c) const {
+        constexpr int E = Vec<T>::kElems;
+        if (!VECTOR) return c / piece_elems() == piece && c % THREADS == static_cast<int>(threadIdx.x);
+        const int v = c - span.head;
+        if (v < 0 || v >= span.nvec * E)
+            return piece == 0 && (c < span.head ? c : c - span.nvec * E) == static_cast<int>(threadIdx.x);
+        return v / piece_elems() == piece && v / E % THREADS == static_cast<int>(threadIdx.x);
+    }
+    // whether it is this CTA's
+    __device__ __forceinline__ bool holds(int c) const {
+        if (!VECTOR) return c / piece_elems() == piece;
+        const int v = c - span.head;
+        if (v < 0 || v >= span.nvec * Vec<T>::kElems) return piece == 0;
+        return v / piece_elems() == piece;
+    }
+
+    // The piece's first chunk, on its way while the caller sets up; `run` takes it.
+    __device__ __forceinline__ void fetch(int it, uint4 (&v)[U]) const {
+        const int i0 = it * kVecs + static_cast<int>(threadIdx.x);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            v[u] = i0 + u * THREADS < span.nvec ? load_stream(span.vectors() + i0 + u * THREADS) : masked_vec<T>();
+    }
+    __device__ __forceinline__ void first_chunk(uint4 (&v)[U]) const {
+        if (VECTOR) fetch(piece * chunks, v);
+    }
+
+    template <typename F>
+    __device__ __forceinline__ void run(bool zero, uint4 (&v)[U], F&& f) const {
+        constexpr int E = Vec<T>::kElems;
+        if (!VECTOR) {
+            const int first = piece * piece_elems(), last = min(cols, first + piece_elems());
+            for (int i = first + static_cast<int>(threadIdx.x); i < last; i += THREADS)
+                Vec<T>::store(out + i, zero ? 0.0f : f(make_float2(Vec<T>::load(x + i), 0.0f)).x);
+            return;
+        }
+        uint4* out_vec = reinterpret_cast<uint4*>(out + span.head);
+        if (piece == 0 && static_cast<int>(threadIdx.x) < span.edges) {
+            const int i = span.edge_offset(threadIdx.x);
+            Vec<T>::store(out + i, zero ? 0.0f : f(make_float2(Vec<T>::load(x + i), 0.0f)).x);
+        }
+        const int from = piece * chunks, to = min(from + chunks, chunks_of<T, THREADS, U>(span));
+        if (zero) {
+            for (int i = from * kVecs + static_cast<int>(threadIdx.x); i < min(to * kVecs, span.nvec); i += THREADS)
+                __stcs(out_vec + i, make_uint4(0, 0, 0, 0));
+            return;
+        }
+        for (int it = from; it < to; ++it) {
+            if (it > from) fetch(it, v);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float y[E];
+                Vec<T>::unpack(v[u], y);
+#pragma unroll
+                for (int j = 0; j < E; j += 2) {
+                    const float2 r = f(make_float2(y[j], y[j + 1]));
+                    y[j] = r.x;
+                    y[j + 1] = r.y;
+                }
+                const int i = it * kVecs + static_cast<int>(threadIdx.x) + u * THREADS;
+                if (i < span.nvec) __stcs(out_vec + i, Vec<T>::pack(y));
+            }
+        }
+    }
+};
+
 // ---------------------------------------------------------------------------
 // the softmax record
 // ---------------------------------------------------------------------------
