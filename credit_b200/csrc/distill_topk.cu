@@ -65,11 +65,10 @@ struct TeacherList {
     int any;                   // some place is used
 };
 
-// Warp 0 reads the list; all threads see it behind a barrier that the caller places.
+// One warp reads the list; the others see it behind a barrier that the caller places.
 template <bool TAIL>
 __device__ __forceinline__ void load_list(const DistillArgs& a, int64_t row, TeacherList& l) {
-    if (threadIdx.x >= 32) return;
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & 31;
     float v[kPerLane];
     bool bad = false, any = false;
     float top = -CUDART_INF_F;
@@ -108,125 +107,89 @@ __device__ __forceinline__ void load_list(const DistillArgs& a, int64_t row, Tea
     }
 }
 
-// ---------------------------------------------------------------------------
-// forward: one cluster per row, the row read once
-// ---------------------------------------------------------------------------
+// What one thread holds of a row while it streams by, and how its listed columns are kept out of the sums.
 template <typename T, bool TAIL>
-__global__ void __launch_bounds__(kThreads, 4) distill_topk_kernel(const DistillArgs a) {
-    __shared__ SoftmaxRecord warp_records[kThreads / 32];
-    __shared__ SoftmaxRecord records[kMaxClusterSize];
-    __shared__ TeacherList list;
-    extern __shared__ __align__(16) uint32_t bitmap[];   // TAIL: one bit per element of the slice, vectors first
+struct DistillPass {
+    static constexpr int E = Vec<T>::kElems;
+    const RowSpan<T>& span;
+    uint32_t* bitmap;   // TAIL: one bit per element of the slice, vectors first, then edges
+    float k2;
+    SoftmaxRecord rec;
 
-    constexpr int E = Vec<T>::kElems;
-    const uint32_t rank = cluster_cta_rank(), nranks = cluster_cta_count();
-    const int64_t row = blockIdx.x / nranks;
-    const int tid = threadIdx.x;
-    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-    const int start = static_cast<int>(rank) * a.slice;
-    const int local = max(0, min(a.slice, a.cols - start));
-    const RowSpan<T> span(x, start, local);
-    const float k2 = a.inv_t * kLog2e;
+    __device__ __forceinline__ DistillPass(const RowSpan<T>& s, uint32_t* b, float k2_) : span(s), bitmap(b), k2(k2_), rec(empty_record()) {}
 
-    load_list<TAIL>(a, row, list);
-    if (TAIL)
-        for (int i = tid; i < a.bitmap_words; i += kThreads) bitmap[i] = 0;
-    __syncthreads();
-    if (!list.bad && (TAIL ? !list.any : list.mass == 0.0)) {
-        // no teacher in this row: nothing is read (the whole cluster leaves here)
-        if (rank == 0) {
-            if (tid == 0) a.loss[row] = 0.0f;
-            if (tid < kStats) a.stats[row * kStats + tid] = tid == 0 ? -CUDART_INF_F : 0.0f;   // no gradient
-        }
-        return;
-    }
-    cluster_arrive_release();
-    // bit of an element: its place in the vectors, or behind them for the edges
-    auto place_of = [&](int offset) {
-        const int v = offset - span.head;
+    // a column's word and bit; the column must lie in the slice
+    __device__ __forceinline__ int place_of(int column) const {
+        const int offset = column - span.start, v = offset - span.head;
         if (v >= 0 && v < span.nvec * E) return v;
         return span.nvec * E + (offset < span.head ? offset : offset - span.nvec * E);
-    };
-    float listed = -CUDART_INF_F;   // the student's logit at list entry tid, for the row's finish in rank 0
-    if (tid < a.top_k && list.column[tid] >= 0) {
-        const int offset = list.column[tid] - start;
-        if (TAIL && offset >= 0 && offset < local) {
-            const int p = place_of(offset);
-            atomicOr(&bitmap[p >> 5], 1u << (p & 31));
-        }
-        if (rank == 0) listed = Vec<T>::load(x + list.column[tid]);
     }
-    if (TAIL) __syncthreads();
+    __device__ __forceinline__ bool holds(int column) const { return column >= span.start && column < span.start + span.local; }
+    // true when the column was marked before
+    __device__ __forceinline__ bool mark(int column) const {
+        const int p = place_of(column);
+        return atomicOr(&bitmap[p >> 5], 1u << (p & 31)) >> (p & 31) & 1u;
+    }
 
-    SoftmaxRecord rec = empty_record();
-    auto add = [&](auto& v) {
-        constexpr int U = sizeof(v) / sizeof(uint4);
-        float part[U];
-        const float top = chunk_max<T, U>(v, part);
-        accumulate<T, U, false>(v, top, k2, rec);
-    };
-    // listed elements of a vector become masked ones
-    auto hide = [&](uint4& v, uint32_t bits) {
-        float y[E];
-        Vec<T>::unpack(v, y);
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (bits >> j & 1u) y[j] = -CUDART_INF_F;
-        v = Vec<T>::pack(y);
-    };
-    const float edge = edge_element(span);
-    stream_chunks<T, kThreads, kUnroll>(span, 0, chunks_of<T, kThreads, kUnroll>(span), [&](uint4 (&v)[kUnroll], int first) {
+    template <int U>
+    __device__ __forceinline__ void add(const uint4 (&v)[U]) {
+        accumulate<T, U, false>(v, chunk_max<T, U>(v), k2, rec);
+    }
+    template <int U>
+    __device__ __forceinline__ void take(uint4 (&v)[U], int first) {
         if (TAIL) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const int p = (first + u * kThreads) * E;
-                const uint32_t bits = p < span.nvec * E ? bitmap[p >> 5] >> (p & 31) & ((1u << E) - 1u) : 0u;
-                if (bits != 0) hide(v[u], bits);
+            for (int u = 0; u < U; ++u) {
+                // a vector's bits: a byte (a nibble) of the map
+                const int i = first + u * kThreads;
+                uint32_t bits = 0;
+                if (i < span.nvec)
+                    bits = E == 8 ? reinterpret_cast<const uint8_t*>(bitmap)[i]
+                                  : reinterpret_cast<const uint8_t*>(bitmap)[i >> 1] >> (i & 1) * 4 & 15u;
+                if (bits != 0) {
+                    float y[E];
+                    Vec<T>::unpack(v[u], y);
+#pragma unroll
+                    for (int j = 0; j < E; ++j)
+                        if (bits >> j & 1u) y[j] = -CUDART_INF_F;
+                    v[u] = Vec<T>::pack(y);
+                }
             }
         }
         add(v);
-    });
-    if (span.edges > 0) {
-        const int p = span.nvec * E + tid;
-        const bool hidden = TAIL && tid < span.edges && (bitmap[p >> 5] >> (p & 31) & 1u) != 0;
-        uint4 v[1] = {Vec<T>::single(hidden ? -CUDART_INF_F : edge)};
+    }
+    __device__ __forceinline__ void take_edges(float edge) {
+        if (span.edges == 0) return;
+        const int p = span.nvec * E + static_cast<int>(threadIdx.x);
+        const bool hidden = TAIL && static_cast<int>(threadIdx.x) < span.edges && (bitmap[p >> 5] >> (p & 31) & 1u) != 0;
+        const uint4 v[1] = {Vec<T>::single(hidden ? -CUDART_INF_F : edge)};
         add(v);
     }
-    rec = cta_record<kThreads>(rec, warp_records, k2);
-    cluster_wait_acquire();
-    if (nranks > 1) {
-        if (rank != 0 && tid == 0) {
-            const uint32_t to = map_to_rank(smem_u32(&records[rank]), 0);
-            st_cluster_f32(to, rec.m);
-            st_cluster_f32(to + 4, rec.s);
-            st_cluster_f32(to + 8, rec.e);
-        }
-        cluster_sync_all();
-        if (rank != 0) return;
-    }
-    // rank 0, warp 0 finishes the row; lane l holds list entries l, l + 32, ... (their logits come
-    // through shared memory)
-    __shared__ float student[kMaxList];
-    if (tid < kMaxList) student[tid] = listed;
-    __syncthreads();
-    if (tid >= 32) return;
-    if (nranks > 1) {
-        if (tid == 0) records[0] = rec;
-        __syncwarp();
-        rec = warp_record<kMaxClusterSize>(tid < static_cast<int>(nranks) ? records[tid] : empty_record(), k2);
-    }
-    SoftmaxRecord all = rec;   // with a tail `rec` covers the columns outside the list
+};
+
+__device__ __forceinline__ void write_no_teacher(const DistillArgs& a, int64_t row) {
+    if (threadIdx.x == 0) a.loss[row] = 0.0f;
+    if (threadIdx.x < kStats) a.stats[row * kStats + threadIdx.x] = threadIdx.x == 0 ? -CUDART_INF_F : 0.0f;   // no gradient
+}
+
+// A row's results, by warp 0: `rec` over the row's columns (with a tail: those outside the list), the student's
+// logits at the list's entries (-inf for unused ones). Lane l holds entries l, l + 32, ...
+template <bool TAIL>
+__device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, const TeacherList& list, const float* student,
+                                           bool repeats, const SoftmaxRecord& rec, float k2) {
+    const int lane = threadIdx.x;
+    SoftmaxRecord all = rec;
     if (TAIL) {
         // the listed columns, each once: a repeated column counts where it appears first
         float y[kPerLane];
         float top = -CUDART_INF_F;
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i) {
-            const int k = tid + 32 * i;
-            const int c = list.column[k];
-            bool repeated = false;
-            for (int j = 0; j < k; ++j) repeated |= list.column[j] == c;
-            y[i] = c < 0 || repeated ? -CUDART_INF_F : student[k];
+            const int k = lane + 32 * i;
+            y[i] = student[k];
+            if (repeats)
+                for (int j = 0; j < k; ++j)
+                    if (list.column[j] == list.column[k]) y[i] = -CUDART_INF_F;
             top = max_nan(top, y[i]);
         }
         SoftmaxRecord mine = empty_record();
@@ -260,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_topk_kernel(const Distill
     double loss = 0.0;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-        const int k = tid + 32 * i;
+        const int k = lane + 32 * i;
         const float logw = list.value[k] - log_norm;
         const float w = expf(logw);
         if (list.column[k] >= 0 && w != 0.0f) {
@@ -269,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_topk_kernel(const Distill
         }
     }
     loss = warp_sum_f64(loss);
-    if (tid == 0) {
+    if (lane == 0) {
         if (TAIL && rest > 0.0f) {
             const float log_rest_q = (rec.m - all.m) * a.inv_t + (tail_log_sum - log_sum);
             loss += static_cast<double>(rest) * (logf(rest) - log_rest_q);
@@ -284,6 +247,76 @@ __global__ void __launch_bounds__(kThreads, 4) distill_topk_kernel(const Distill
         s[4] = log_norm;
         s[5] = rest;
     }
+}
+
+// ---------------------------------------------------------------------------
+// forward: one cluster per row, the row read once
+// ---------------------------------------------------------------------------
+template <typename T, bool TAIL>
+__global__ void __launch_bounds__(kThreads, 4) distill_topk_kernel(const DistillArgs a) {
+    __shared__ SoftmaxRecord warp_records[kThreads / 32];
+    __shared__ SoftmaxRecord records[kMaxClusterSize];   // rank 0: one per CTA; e = 1: a column repeats there
+    __shared__ TeacherList list;
+    __shared__ float student[kMaxList];
+    extern __shared__ __align__(16) uint32_t bitmap[];
+
+    const uint32_t rank = cluster_cta_rank(), nranks = cluster_cta_count();
+    const int64_t row = blockIdx.x / nranks;
+    const int tid = threadIdx.x;
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    const int start = static_cast<int>(rank) * a.slice;
+    const RowSpan<T> span(x, start, max(0, min(a.slice, a.cols - start)));
+    DistillPass<T, TAIL> pass(span, bitmap, a.inv_t * kLog2e);
+
+    if (tid < 32) load_list<TAIL>(a, row, list);
+    if (TAIL)
+        for (int i = tid; i < a.bitmap_words; i += kThreads) bitmap[i] = 0;
+    __syncthreads();
+    if (!list.bad && (TAIL ? !list.any : list.mass == 0.0)) {
+        // no teacher in this row: nothing is read (the whole cluster leaves here)
+        if (rank == 0) write_no_teacher(a, row);
+        return;
+    }
+    cluster_arrive_release();
+    bool repeats = false;
+    if (tid < kMaxList) {
+        const int column = tid < a.top_k ? list.column[tid] : -1;
+        if (TAIL && pass.holds(column)) repeats = pass.mark(column);
+        if (rank == 0) student[tid] = column >= 0 ? Vec<T>::load(x + column) : -CUDART_INF_F;
+    }
+    if (TAIL) repeats = __syncthreads_or(repeats);
+
+    const float edge = edge_element(span);
+    stream_chunks<T, kThreads, kUnroll>(span, 0, chunks_of<T, kThreads, kUnroll>(span),
+                                        [&](uint4 (&v)[kUnroll], int first) { pass.take(v, first); });
+    pass.take_edges(edge);
+    SoftmaxRecord rec = cta_record<kThreads>(pass.rec, warp_records, pass.k2);
+    cluster_wait_acquire();
+    if (nranks > 1) {
+        if (rank != 0 && tid == 0) {
+            const uint32_t to = map_to_rank(smem_u32(&records[rank]), 0);
+            st_cluster_f32(to, rec.m);
+            st_cluster_f32(to + 4, rec.s);
+            st_cluster_f32(to + 8, repeats ? 1.0f : 0.0f);
+        }
+        cluster_sync_all();
+        if (rank != 0) return;
+    }
+    if (tid >= 32) return;
+    if (nranks > 1) {
+        if (tid == 0) records[0] = rec;
+        __syncwarp();
+        if (tid < static_cast<int>(nranks)) {
+            rec = records[tid];
+            if (tid > 0 && rec.e != 0.0f) repeats = true;
+            rec.e = 0.0f;
+        } else {
+            rec = empty_record();
+        }
+        repeats = __any_sync(0xffffffffu, repeats);
+        rec = warp_record<kMaxClusterSize>(rec, pass.k2);
+    }
+    finish_row<TAIL>(a, row, list, student, repeats, rec, pass.k2);
 }
 
 // ---------------------------------------------------------------------------
@@ -401,14 +434,15 @@ int forward(const void* logits, int64_t ld, const int64_t* index, const float* t
     a.loss = loss;
     a.stats = stats;
     a.cols = static_cast<int>(cols);
+    a.inv_t = 1.0f / temperature;
+    a.status = ctx.status;
+    void* args[] = {&a};
     a.slice = row_slice(cols, cluster);
     if (tail != 0 && a.slice > (1 << 20)) {   // the bitmap of a slice: at most 128 KiB
         cluster = cluster < 4 ? 4 : cluster;
         a.slice = row_slice(cols, cluster);
     }
     a.bitmap_words = tail != 0 ? (a.slice + 31) / 32 : 0;
-    a.inv_t = 1.0f / temperature;
-    a.status = ctx.status;
     const void* func;
     if (dtype == CREDIT_BF16)
         func = tail ? reinterpret_cast<const void*>(&distill_topk_kernel<__nv_bfloat16, true>)
@@ -418,7 +452,6 @@ int forward(const void* logits, int64_t ld, const int64_t* index, const float* t
                     : reinterpret_cast<const void*>(&distill_topk_kernel<float, false>);
     rc = prepare_kernel(ctx, func);
     if (rc != CREDIT_OK) return rc;
-    void* args[] = {&a};
     return launch_kernel(func, rows * cluster, kThreads, cluster, a.bitmap_words * 4, stream, args);
 }
 

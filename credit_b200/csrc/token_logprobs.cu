@@ -36,6 +36,56 @@ struct LogprobArgs {
     int* status;
 };
 
+// An ignored row, by the threads of one CTA.
+template <bool ENTROPY, bool TOP>
+__device__ __forceinline__ void write_ignored(const LogprobArgs& a, int64_t row) {
+    const int tid = threadIdx.x;
+    if (tid == 0) {
+        a.logprob[row] = 0.0f;
+        a.stats[2 * row] = a.stats[2 * row + 1] = 0.0f;
+        if (ENTROPY) a.entropy[row] = 0.0f;
+    }
+    if (TOP && tid < a.top_k) {
+        a.top_logprob[row * a.top_k + tid] = -CUDART_INF_F;
+        a.top_index[row * a.top_k + tid] = -1;
+    }
+}
+
+// The target's logit, by one thread; NaN when there is none to read.
+template <typename T>
+__device__ __forceinline__ float target_logit(const LogprobArgs& a, const T* x, int64_t target) {
+    if (a.targets == nullptr) return CUDART_NAN_F;
+    if (target < a.cols) return Vec<T>::load(x + target);
+    atomicOr(a.status, kStatusBadIndex);
+    return CUDART_NAN_F;
+}
+
+// A row's scalars from its record, by one thread; returns its log sum.
+template <bool ENTROPY>
+__device__ __forceinline__ float write_row(const LogprobArgs& a, int64_t row, const SoftmaxRecord& rec, int64_t target,
+                                           float picked, float k2) {
+    const bool broken = is_broken(rec.m), empty = rec.m == -CUDART_INF_F;
+    const float log_sum = broken ? CUDART_NAN_F : (empty ? 0.0f : log_sum_of(rec, k2));
+    a.stats[2 * row] = rec.m;
+    a.stats[2 * row + 1] = log_sum;
+    if (a.targets != nullptr)
+        a.logprob[row] = empty && target < a.cols ? -CUDART_INF_F : (picked - rec.m) * a.inv_t - log_sum;
+    if (ENTROPY) a.entropy[row] = broken ? CUDART_NAN_F : (empty ? 0.0f : logf(rec.s) - kLn2 * (rec.e / rec.s));
+    return log_sum;
+}
+
+// The sorted alternatives in t.keys, by the threads of one CTA.
+__device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, const TopBuffer& t, float row_max,
+                                          float row_log_sum) {
+    const int tid = threadIdx.x;
+    if (tid >= a.top_k) return;
+    const int64_t at = row * a.top_k + tid;
+    const bool present = tid < t.fill;
+    const uint64_t key = present ? t.keys[tid] : 0;
+    a.top_logprob[at] = present ? (key_value(key) - row_max) * a.inv_t - row_log_sum : -CUDART_INF_F;
+    a.top_index[at] = present ? key_column(key) : -1;
+}
+
 // ---------------------------------------------------------------------------
 // forward: one cluster per row, the row read once
 // ---------------------------------------------------------------------------
@@ -56,29 +106,12 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
     if (a.targets != nullptr) {
         target = a.targets[row];
         if (target < 0) {   // ignored row: nothing is read (the whole cluster leaves here)
-            if (rank == 0) {
-                if (tid == 0) {
-                    a.logprob[row] = 0.0f;
-                    a.stats[2 * row] = a.stats[2 * row + 1] = 0.0f;
-                    if (ENTROPY) a.entropy[row] = 0.0f;
-                }
-                if (TOP && tid < a.top_k) {
-                    a.top_logprob[row * a.top_k + tid] = -CUDART_INF_F;
-                    a.top_index[row * a.top_k + tid] = -1;
-                }
-            }
+            if (rank == 0) write_ignored<ENTROPY, TOP>(a, row);
             return;
         }
     }
     cluster_arrive_release();   // "this CTA runs": its shared memory may be written from now on
-    float picked = CUDART_NAN_F;
-    if (a.targets != nullptr && rank == 0 && tid == 0) {
-        if (target < a.cols) {
-            picked = Vec<T>::load(x + target);
-        } else {
-            atomicOr(a.status, kStatusBadIndex);
-        }
-    }
+    const float picked = rank == 0 && tid == 0 ? target_logit(a, x, target) : 0.0f;
     if (TOP && tid == 0) init_top_buffer(t);
 
     const int start = static_cast<int>(rank) * a.slice;
@@ -87,36 +120,23 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
     const float k2 = a.inv_t * kLog2e;
     const float edge = edge_element(span);
     SoftmaxRecord rec = empty_record();
-    TopCollector<T> collector(t, a.top_k);
     const int chunks = chunks_of<T, kThreads, kUnroll>(span);
-    int from = 0, to = TOP ? 1 : chunks;
-    do {
-        stream_chunks<T, kThreads, kUnroll>(span, from, min(to, chunks), [&](const uint4 (&v)[kUnroll], int first) {
-            float part[kUnroll];
-            const float top = chunk_max<T>(v, part);
-            if (TOP) {
-                constexpr int kStride = kThreads * Vec<T>::kElems;
-                const int column = span.vector_column(first);
-                if (from == 0) collector.first_threshold(v, part, top, column, kStride);
-                collector.note_chunk(part, top, first, column, kStride);
-            }
-            accumulate<T, kUnroll, ENTROPY>(v, top, k2, rec);
-        });
-        from = to;
-        to *= 4;
-        if (TOP && from < chunks) collector.tighten(span);
-    } while (from < chunks);
+    TopCollector<T, kUnroll> collector(t, a.top_k, chunks);
+    stream_chunks<T, kThreads, kUnroll>(span, 0, chunks, [&](const uint4 (&v)[kUnroll], int first) {
+        const float top = chunk_max<T>(v);
+        if (TOP) collector.add(top, first / (kThreads * kUnroll));
+        accumulate<T, kUnroll, ENTROPY>(v, top, k2, rec);
+    });
     if (span.edges > 0) {
-        if (TOP) {
-            if (chunks == 0) __syncthreads();   // the buffer's first use
-            if (tid < span.edges) collector.offer(edge, span.start + span.edge_offset(tid));
-        }
         const uint4 v[1] = {Vec<T>::single(edge)};
         accumulate<T, 1, ENTROPY>(v, edge, k2, rec);
     }
-
-    rec = cta_record<kThreads>(rec, warp_records, k2);
-    if (TOP) collector.finish(span);
+    const float thread_max = rec.m;
+    rec = cta_record<kThreads>(rec, warp_records, k2);   // its barrier also lies behind the buffer's set-up
+    if (TOP) {
+        if (tid < span.edges) collector.add_edge(edge, span.start + span.edge_offset(tid));
+        collector.finish(span, thread_max);
+    }
     cluster_wait_acquire();
     if (nranks > 1) {
         // rank 0 gathers the records, and the lists behind its own buffer
@@ -140,25 +160,12 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
     }
 
     if (tid == 0) {
-        const bool broken = is_broken(rec.m), empty = rec.m == -CUDART_INF_F;
-        const float log_sum = broken ? CUDART_NAN_F : (empty ? 0.0f : log_sum_of(rec, k2));
         row_max = rec.m;
-        row_log_sum = log_sum;
-        a.stats[2 * row] = rec.m;
-        a.stats[2 * row + 1] = log_sum;
-        if (a.targets != nullptr)
-            a.logprob[row] = empty && target < a.cols ? -CUDART_INF_F : (picked - rec.m) * a.inv_t - log_sum;
-        if (ENTROPY) a.entropy[row] = broken ? CUDART_NAN_F : (empty ? 0.0f : logf(rec.s) - kLn2 * (rec.e / rec.s));
+        row_log_sum = write_row<ENTROPY>(a, row, rec, target, picked, k2);
     }
     if (TOP) {
         __syncthreads();
-        if (tid < a.top_k) {
-            const int64_t at = row * a.top_k + tid;
-            const bool present = tid < t.fill;
-            const uint64_t key = present ? t.keys[tid] : 0;
-            a.top_logprob[at] = present ? (key_value(key) - row_max) * a.inv_t - row_log_sum : -CUDART_INF_F;
-            a.top_index[at] = present ? key_column(key) : -1;
-        }
+        write_top(a, row, t, row_max, row_log_sum);
     }
 }
 

@@ -1,20 +1,20 @@
-// The k largest of a row slice that is read once: vectors that may hold one of them are noted in shared
-// memory as they stream by (their number, nothing more: a note costs a dozen instructions, a key of an
-// element several times that), a threshold (always the key of a real element that k elements reach) keeps
-// the rest out. Between intervals of chunks the noted vectors are read again, a thread each, and the keys
-// of their elements compete.
+// The k largest of a row slice that is read once. While it streams by, every thread stores the maximum of each
+// group of its elements (32 bf16 or 16 fp32 a chunk; as many chunks a group as make at most 16 groups): one store
+// and nothing else. At the end every warp takes its ceil(k / 8)-th largest thread maximum; the smallest of the
+// eight has k elements that reach it, about 50 (k = 20) to 250 (k = 128) groups do, and those are read again: their
+// elements that reach it compete by rank.
 //
 // Order. An element is the 64-bit key (monotone image of its value, complement of its column): larger
 // keys first is "value descending, column ascending", all keys of a row differ, so the chosen set
 // does not depend on the order in which threads append. NaN ranks above +inf, -0 equals +0, -inf is
 // never an element (its image lies under kLowestKey).
 //
-// The threshold starts from the threads' first-chunk maxima: every warp takes its ceil(k / 8)-th largest,
-// and the smallest of the eight has k elements that reach it. On rows in no particular order it lets about
-// 50 (k = 20) to 250 (k = 128) elements of a chunk through. It is tightened to the k-th largest candidate
-// after chunks 1, 4, 16, 64, ...; each later interval then notes about 3k vectors, so 1024 notes hold every
-// k up to 128. A row that brings more (sorted ascending, say) overflows; its slice is then searched by
+// A slice with more groups or elements at the threshold than there are places (thousands of ties) is searched by
 // the digit-by-digit selection straight from global memory, at most 8 more reads of it.
+//
+// What was measured before this form, 4096 rows of 131072 bf16, k = 20 (164 us without alternatives): a running
+// threshold made exact after chunks 1, 4, 16 by all threads 270 us; kept by the warps without barriers 315 us: noting
+// candidates costs a warp some 100 instructions in most chunks, whoever holds the threshold.
 #pragma once
 
 #include "vocab_rows.cuh"
@@ -24,7 +24,7 @@ namespace credit {
 constexpr int kMaxTop = 128;
 constexpr int kTopThreads = 256;
 constexpr int kTopCapacity = 2048;
-constexpr int kTopNotes = 1024;
+constexpr int kTopGroups = 16;   // a thread's
 constexpr uint64_t kLowestKey = 0x0080000000000000ull;   // the image of -FLT_MAX, any column
 
 __device__ __forceinline__ uint64_t element_key(float x, int column) {
@@ -38,17 +38,18 @@ struct TopBuffer {
     unsigned long long keys[kTopCapacity];
     unsigned int hist[256];
     unsigned long long lowest;   // smallest kept key
-    unsigned long long floor[kTopThreads / 32];   // first threshold of each warp
+    float group[kTopGroups][kTopThreads];   // maxima
+    unsigned int floor[kTopThreads / 32];   // image of each warp's share of the threshold
     unsigned int differ[2];      // bits in which the keys differ (high, low word); zero between calls
-    int notes[kTopNotes];        // vectors of the slice
-    int noted;                   // (may exceed the places, like count)
+    int noted[kTopCapacity];     // groups that reach the threshold
+    int notes;                   // (may exceed the places, like count)
     int count;                   // candidates appended
     int fill, digit, above, here;
 };
 
 // By one thread, before the first barrier.
 __device__ __forceinline__ void init_top_buffer(TopBuffer& t) {
-    t.count = t.noted = 0;
+    t.count = t.notes = 0;
     t.differ[0] = t.differ[1] = 0;
 }
 
@@ -228,133 +229,86 @@ __device__ __noinline__ void select_from_slice(const T* first, int start, int lo
     __syncthreads();
 }
 
-// One CTA's candidates while its slice streams by.
-template <typename T>
+// One CTA's groups while its slice streams by, in chunks of U vectors a thread.
+template <typename T, int U>
 struct TopCollector {
+    static constexpr int E = Vec<T>::kElems;
     TopBuffer& t;
     const int k;
-    uint64_t key;    // threshold
-    float value;     // its value (+inf when that is NaN, which then lets NaN and +inf through)
-    bool overflow;
+    int chunks, per_group;
+    float running;
 
-    __device__ __forceinline__ TopCollector(TopBuffer& t_, int k_) : t(t_), k(k_), key(kLowestKey), overflow(false) {
-        set_threshold(kLowestKey);
-    }
+    __device__ __forceinline__ TopCollector(TopBuffer& t_, int k_, int chunks_)
+        : t(t_), k(k_), chunks(chunks_), per_group((chunks_ + kTopGroups - 1) / kTopGroups), running(-INFINITY) {}
 
-    __device__ __forceinline__ void set_threshold(uint64_t to) {
-        if (to > key) key = to;
-        value = key_value(key);
-        if (value != value) value = CUDART_INF_F;
-    }
-
-    // The first chunk: see the top of the file. `column` is that of the thread's first vector.
-    template <int U>
-    __device__ __forceinline__ void first_threshold(const uint4 (&v)[U], const float (&part)[U], float top, int column,
-                                                    int stride) {
-        uint32_t hi = 0, lo = 0;   // this thread's largest element
-        if (!(top < value)) {
-            const bool nan = top != top;
-            int at = 0;
-#pragma unroll
-            for (int u = U - 1; u >= 0; --u)
-                if (nan ? part[u] != part[u] : part[u] == top) at = u;
-            float x[Vec<T>::kElems];
-            Vec<T>::unpack(pick(v, at), x);
-            int j = 0;
-#pragma unroll
-            for (int i = Vec<T>::kElems - 1; i >= 0; --i)
-                if (nan ? x[i] != x[i] : x[i] == top) j = i;
-            hi = ordered_image(top);
-            lo = 0xffffffffu - static_cast<uint32_t>(column + at * stride + j);
+    // The thread's maximum of chunk `it`.
+    __device__ __forceinline__ void add(float top, int it) {
+        running = max_nan(running, top);
+        const int g = per_group == 1 ? it : it / per_group;
+        if (per_group == 1 || it + 1 == (g + 1) * per_group || it + 1 == chunks) {
+            t.group[g][threadIdx.x] = running;
+            running = -CUDART_INF_F;
         }
-        const int lane = threadIdx.x & 31;
-        bool taken = false;
-        uint32_t m = 0;
-#pragma unroll 1
-        for (int i = 0; i < (k + 7) / 8; ++i) {
-            m = __reduce_max_sync(0xffffffffu, taken ? 0u : hi);
-            const unsigned int same = __ballot_sync(0xffffffffu, !taken && hi == m);
-            taken |= lane == __ffs(same) - 1;
-        }
-        const uint32_t low = __reduce_min_sync(0xffffffffu, taken && hi == m ? lo : 0xffffffffu);
-        if (lane == 0) t.floor[threadIdx.x >> 5] = (static_cast<uint64_t>(m) << 32) | low;
-        __syncthreads();
-        uint64_t least = t.floor[0];
-#pragma unroll
-        for (int w = 1; w < kTopThreads / 32; ++w) least = t.floor[w] < least ? t.floor[w] : least;
-        set_threshold(least);
     }
 
     __device__ __forceinline__ void offer(float x, int column) {
-        if (x < value) return;
-        const uint64_t c = element_key(x, column);
-        if (c < key) return;
         const int at = atomicAdd(&t.count, 1);
-        if (at < kTopCapacity) t.keys[at] = c;
+        if (at < kTopCapacity) t.keys[at] = element_key(x, column);
     }
 
-    // v[at] without an indexed register file
-    template <int U>
-    __device__ __forceinline__ static uint4 pick(const uint4 (&v)[U], int at) {
-        uint4 r = v[0];
-#pragma unroll
-        for (int u = 1; u < U; ++u)
-            if (at == u) r = v[u];
-        return r;
+    // An element outside the vectors competes in any case.
+    __device__ __forceinline__ void add_edge(float x, int column) {
+        if (x != -CUDART_INF_F) offer(x, column);
     }
 
-    // Notes the vectors of a chunk that reach the threshold; among equals of its value only those that start at
-    // its column or before it.
-    template <int U>
-    __device__ __forceinline__ void note_chunk(const float (&part)[U], float top, int first, int column, int stride) {
-        if (top < value) return;
-        const uint32_t last = 0xffffffffu - static_cast<uint32_t>(key);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (!(part[u] <= value) || (part[u] == value && static_cast<uint32_t>(column + u * stride) <= last)) {
-                const int at = atomicAdd(&t.noted, 1);
-                if (at < kTopNotes) t.notes[at] = first + u * kTopThreads;
+    // The k largest of the slice in keys[0, fill), sorted, behind a barrier. `thread_max`: over all of the
+    // thread's elements, edges included.
+    __device__ __forceinline__ void finish(const RowSpan<T>& span, float thread_max) {
+        const int tid = threadIdx.x, lane = tid & 31;
+        const uint32_t mine = ordered_image(thread_max);
+        uint32_t m = 0;
+        bool taken = false;
+#pragma unroll 1
+        for (int i = 0; i < (k + 7) / 8; ++i) {
+            m = __reduce_max_sync(0xffffffffu, taken ? 0u : mine);
+            taken |= lane == __ffs(__ballot_sync(0xffffffffu, !taken && mine == m)) - 1;
+        }
+        if (lane == 0) t.floor[tid >> 5] = m;
+        __syncthreads();
+        const uint32_t least = max(__reduce_min_sync(0xffffffffu, t.floor[lane & (kTopThreads / 32 - 1)]),
+                                   static_cast<uint32_t>(kLowestKey >> 32));
+        const float floor = image_value(least);   // NaN: only NaN reaches it
+        const bool nan = floor != floor;
+        const int groups = (chunks + per_group - 1) / max(per_group, 1);
+#pragma unroll 1
+        for (int g = 0; g < groups; ++g) {
+            const float x = t.group[g][tid];
+            if (nan ? x != x : !(x < floor)) {
+                const int at = atomicAdd(&t.notes, 1);
+                if (at < kTopCapacity) t.noted[at] = g * kTopThreads + tid;
             }
         }
-    }
-
-    // The elements of the noted vectors become candidates. All threads; ends with a barrier.
-    __device__ __forceinline__ void expand(const RowSpan<T>& span) {
         __syncthreads();
-        const int n = t.noted;
-        __syncthreads();   // everyone has read it
-        if (n > kTopNotes) overflow = true;
-        if (threadIdx.x == 0) t.noted = 0;
+        const int notes = t.notes, vectors = U * per_group;
+        bool overflow = notes > kTopCapacity;
         if (!overflow) {
 #pragma unroll 1
-            for (int i = threadIdx.x; i < n; i += kTopThreads) {
-                const int v = t.notes[i], column = span.vector_column(v);
-                float x[Vec<T>::kElems];
+            for (int i = tid; i < notes * vectors; i += kTopThreads) {
+                const int note = t.noted[i / vectors], place = i % vectors;
+                const int v = ((note / kTopThreads * per_group) * U + place) * kTopThreads + note % kTopThreads;
+                if (v >= span.nvec) continue;
+                const int column = span.vector_column(v);
+                float x[E];
                 Vec<T>::unpack(span.vectors()[v], x);
 #pragma unroll
-                for (int j = 0; j < Vec<T>::kElems; ++j) offer(x[j], column + j);
+                for (int j = 0; j < E; ++j)
+                    if (nan ? x[j] != x[j] : !(x[j] < floor)) offer(x[j], column + j);
             }
         }
         __syncthreads();
-        if (t.count > kTopCapacity) overflow = true;
-    }
-
-    // Between intervals of chunks: keep the k largest so far.
-    __device__ __forceinline__ void tighten(const RowSpan<T>& span) {
-        expand(span);
-        const int n = t.count;
-        if (n > k && !overflow) {
-            set_threshold(rank_largest(t, n, k));
-            if (threadIdx.x == 0) t.count = t.fill;
-        }
-        __syncthreads();
-    }
-
-    // The k largest of the slice in keys[0, fill), sorted, behind a barrier.
-    __device__ __forceinline__ void finish(const RowSpan<T>& span) {
-        expand(span);
         int n = t.count;
-        if (overflow) {
+        if (overflow || n > kTopCapacity) {
+            __syncthreads();
             select_from_slice(span.first, span.start, span.local, k, t);
             n = t.fill;
             __syncthreads();

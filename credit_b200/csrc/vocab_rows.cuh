@@ -382,13 +382,10 @@ __device__ __forceinline__ void accumulate(const uint4 (&v)[U], float top, float
 }
 
 template <typename T, int U>
-__device__ __forceinline__ float chunk_max(const uint4 (&v)[U], float (&part)[U]) {
-    float top = -CUDART_INF_F;
+__device__ __forceinline__ float chunk_max(const uint4 (&v)[U]) {
+    float top = Vec<T>::max(v[0]);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        part[u] = Vec<T>::max(v[u]);
-        top = max_nan(top, part[u]);
-    }
+    for (int u = 1; u < U; ++u) top = max_nan(top, Vec<T>::max(v[u]));
     return top;
 }
 

@@ -373,7 +373,7 @@ int credit_token_logprobs_backward(const void* logits, int64_t row_stride, const
  *             outcome that is compared with the student's mass outside the list.
  * loss is fp32 [rows]; stats fp32 [rows, 6] is the state the backward call needs.
  *   - A negative index marks an unused place. A row without a used place (or, with tail = 0,
- *     without teacher mass) has loss 0 and no gradient, and its logits are not read. An
+ *     without teacher mass) has loss 0 and no gradient, whatever its logits are. An
  *     index >= cols sets bit 2 of the device status and gives NaN.
  *   - A column listed twice counts with the sum of its weights' terms in the loss, and once
  *     in the student's mass.

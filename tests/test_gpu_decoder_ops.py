@@ -274,9 +274,10 @@ def _run_logprobs(x, targets, top_k=0, temperature=1.0, cluster=0, ld=None, shif
     return outs
 
 
+# the last two: more rows than twice the SMs, several rows for each persistent CTA
 LOGIT_SHAPES = [(1, 1, None, 0), (3, 2, None, 0), (2, 7, 9, 3), (5, 255, None, 1), (4, 257, 320, 0), (3, 1000, 1024, 8),
                 (2, 4099, None, 5), (3, 8192, None, 0), (2, 8200, 8260, 1), (2, 50001, None, 0), (2, 131072, None, 0),
-                (1, 262147, 262400, 7), (300, 520, None, 0)]
+                (1, 262147, 262400, 7), (300, 520, None, 0), (700, 8200, None, 0), (310, 16411, 16500, 3)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -331,6 +332,27 @@ def test_top_alternatives_of_sorted_and_constant_wide_rows(native_lib, dtype):
     for cluster in (1, 2):
         for top_k in (7, 128):
             _check_logprobs(x, None, _run_logprobs(x, None, top_k, 1.0, cluster), 1.0, top_k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows_with_masks_and_special_values(native_lib, dtype):
+    """The persistent form: rows of every kind next to one another in one CTA's walk."""
+    rows, cols = 900, 9001
+    x, targets = _logits(rows, cols, dtype, 50)
+    x[1::9] = -math.inf
+    x[2::9, 100:] = -math.inf
+    x[3::9] = torch.finfo(dtype).min
+    x[4::9, 17] = NAN
+    x[5::9, 8000] = math.inf
+    x[6::9] = torch.arange(cols).to(dtype)
+    x[7::9] = 1.5
+    targets[8::9] = -1
+    x[8::18] = NAN
+    clean = x.clone()
+    clean[targets < 0] = 0.0
+    for top_k in (0, 20):
+        _check_logprobs(clean, targets, _run_logprobs(x, targets, top_k), 1.0, top_k)
+    assert N.device_status() == 0
 
 
 def test_token_logprobs_ignored_and_bad_targets(native_lib):
@@ -505,6 +527,29 @@ def test_distill_lists_and_masks(native_lib, dtype, tail, cluster):
     x[12, 5] = math.inf
     x[13] = torch.finfo(dtype).min
     _check_distill(x, index, logprob, 1.0, tail, cluster)
+    assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("tail", [True, False])
+def test_distill_many_rows(native_lib, tail):
+    """The persistent form: lists and masks of every kind next to one another in one CTA's walk."""
+    rows, cols, k = 700, 9001, 8
+    x, _ = _logits(rows, cols, torch.bfloat16, 51)
+    index, logprob = _teacher(x, k, 52)
+    index[1::11] = -1
+    index[2::11, 5] = index[2::11, 1]
+    index[2::11, 7] = index[2::11, 1]
+    index[3::11, :] = index[3::11, :1]
+    logprob[4::11] = -math.inf
+    logprob[5::11] = logprob[5::11] + 0.5
+    x[6::11] = -math.inf
+    for r in range(7, rows, 11):
+        keep = x[r, index[r]].clone()
+        x[r] = -math.inf
+        x[r, index[r]] = keep
+    x[8::11, 5] = NAN
+    x[9::11, cols - 1] = math.inf
+    _check_distill(x, index, logprob, 1.0, tail)
     assert N.device_status() == 0
 
 
