@@ -14,6 +14,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "device_context.h"
 #include "vocab_host.h"
@@ -22,7 +23,8 @@
 namespace credit {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;      // forward: eight CTAs an SM (four of 256 threads: 193 instead of 179 us at 4096 x 131072 bf16)
+constexpr int kBwdThreads = 256;
 constexpr int kUnroll = 4;
 constexpr int kMaxList = 128;
 constexpr int kPerLane = kMaxList / 32;
@@ -38,7 +40,7 @@ struct DistillArgs {
     float* stats;            // [rows, 6]
     int cols;
     int slice;
-    int bitmap_words;        // of one slice
+    int map_words;           // of one slice
     float inv_t;
     int* status;
 };
@@ -107,51 +109,57 @@ __device__ __forceinline__ void load_list(const DistillArgs& a, int64_t row, Tea
     }
 }
 
-// What one thread holds of a row while it streams by, and how its listed columns are kept out of the sums.
+// What one thread holds of a row while it streams by, and how its listed columns are kept out of the sums: a map
+// of the slice with a bit for each element of each vector, a thread's bits of one chunk in one word (bf16) or half
+// word (fp32), and behind them a byte for each edge element.
 template <typename T, bool TAIL>
 struct DistillPass {
     static constexpr int E = Vec<T>::kElems;
+    using Bits = std::conditional_t<E == 8, uint32_t, uint16_t>;
     const RowSpan<T>& span;
-    uint32_t* bitmap;   // TAIL: one bit per element of the slice, vectors first, then edges
+    uint32_t* map;
     float k2;
     SoftmaxRecord rec;
 
-    __device__ __forceinline__ DistillPass(const RowSpan<T>& s, uint32_t* b, float k2_) : span(s), bitmap(b), k2(k2_), rec(empty_record()) {}
+    __device__ __forceinline__ DistillPass(const RowSpan<T>& s, uint32_t* m, float k2_) : span(s), map(m), k2(k2_), rec(empty_record()) {}
 
-    // a column's word and bit; the column must lie in the slice
-    __device__ __forceinline__ int place_of(int column) const {
-        const int offset = column - span.start, v = offset - span.head;
-        if (v >= 0 && v < span.nvec * E) return v;
-        return span.nvec * E + (offset < span.head ? offset : offset - span.nvec * E);
+    __device__ __forceinline__ int words() const {   // of vectors
+        return chunks_of<T, kThreads, kUnroll>(span) * kThreads * static_cast<int>(sizeof(Bits)) / 4;
     }
     __device__ __forceinline__ bool holds(int column) const { return column >= span.start && column < span.start + span.local; }
     // true when the column was marked before
     __device__ __forceinline__ bool mark(int column) const {
-        const int p = place_of(column);
-        return atomicOr(&bitmap[p >> 5], 1u << (p & 31)) >> (p & 31) & 1u;
+        const int offset = column - span.start, e = offset - span.head;
+        int word, bit;
+        if (e >= 0 && e < span.nvec * E) {
+            const int v = e / E, chunk = v / (kThreads * kUnroll), u = v / kThreads % kUnroll;
+            const int place = chunk * kThreads + v % kThreads;   // of the thread's bits
+            bit = u * E + e % E;
+            word = E == 8 ? place : place >> 1;
+            if (E == 4) bit += (place & 1) * 16;
+        } else {
+            const int i = offset < span.head ? offset : offset - span.nvec * E;
+            word = words() + i / 4;
+            bit = i % 4 * 8;
+        }
+        return atomicOr(&map[word], 1u << bit) >> bit & 1u;
     }
 
     template <int U>
     __device__ __forceinline__ void add(const uint4 (&v)[U]) {
         accumulate<T, U, false>(v, chunk_max<T, U>(v), k2, rec);
     }
-    template <int U>
-    __device__ __forceinline__ void take(uint4 (&v)[U], int first) {
+    __device__ __forceinline__ void take(uint4 (&v)[kUnroll], int it) {
         if (TAIL) {
+            const uint32_t word = reinterpret_cast<const Bits*>(map)[it * kThreads + threadIdx.x];
+            if (word != 0) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                // a vector's bits: a byte (a nibble) of the map
-                const int i = first + u * kThreads;
-                uint32_t bits = 0;
-                if (i < span.nvec)
-                    bits = E == 8 ? reinterpret_cast<const uint8_t*>(bitmap)[i]
-                                  : reinterpret_cast<const uint8_t*>(bitmap)[i >> 1] >> (i & 1) * 4 & 15u;
-                if (bits != 0) {
+                for (int u = 0; u < kUnroll; ++u) {
                     float y[E];
                     Vec<T>::unpack(v[u], y);
 #pragma unroll
                     for (int j = 0; j < E; ++j)
-                        if (bits >> j & 1u) y[j] = -CUDART_INF_F;
+                        if (word >> (u * E + j) & 1u) y[j] = -CUDART_INF_F;
                     v[u] = Vec<T>::pack(y);
                 }
             }
@@ -160,12 +168,18 @@ struct DistillPass {
     }
     __device__ __forceinline__ void take_edges(float edge) {
         if (span.edges == 0) return;
-        const int p = span.nvec * E + static_cast<int>(threadIdx.x);
-        const bool hidden = TAIL && static_cast<int>(threadIdx.x) < span.edges && (bitmap[p >> 5] >> (p & 31) & 1u) != 0;
+        const int i = threadIdx.x;
+        const bool hidden = TAIL && i < span.edges && (map[words() + i / 4] >> (i % 4 * 8) & 1u) != 0;
         const uint4 v[1] = {Vec<T>::single(hidden ? -CUDART_INF_F : edge)};
         add(v);
     }
 };
+
+// 32-bit words of the map of a slice (whole 16 bytes).
+inline int map_words(int slice, int vec_elems) {
+    const int chunk = kThreads * kUnroll * vec_elems;
+    return (slice + chunk - 1) / chunk * kThreads * vec_elems / 8 + 4;
+}
 
 __device__ __forceinline__ void write_no_teacher(const DistillArgs& a, int64_t row) {
     if (threadIdx.x == 0) a.loss[row] = 0.0f;
@@ -253,12 +267,12 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
 // forward: one cluster per row, the row read once
 // ---------------------------------------------------------------------------
 template <typename T, bool TAIL>
-__global__ void __launch_bounds__(kThreads, 4) distill_topk_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) distill_topk_kernel(const DistillArgs a) {
     __shared__ SoftmaxRecord warp_records[kThreads / 32];
     __shared__ SoftmaxRecord records[kMaxClusterSize];   // rank 0: one per CTA; e = 1: a column repeats there
     __shared__ TeacherList list;
     __shared__ float student[kMaxList];
-    extern __shared__ __align__(16) uint32_t bitmap[];
+    extern __shared__ __align__(16) uint32_t map[];
 
     const uint32_t rank = cluster_cta_rank(), nranks = cluster_cta_count();
     const int64_t row = blockIdx.x / nranks;
@@ -266,11 +280,14 @@ __global__ void __launch_bounds__(kThreads, 4) distill_topk_kernel(const Distill
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
     const int start = static_cast<int>(rank) * a.slice;
     const RowSpan<T> span(x, start, max(0, min(a.slice, a.cols - start)));
-    DistillPass<T, TAIL> pass(span, bitmap, a.inv_t * kLog2e);
+    DistillPass<T, TAIL> pass(span, map, a.inv_t * kLog2e);
+    uint4 ahead[kUnroll];
+    fetch_chunk<T, kThreads, kUnroll>(span, 0, ahead);
+    const float edge = edge_element(span);
 
     if (tid < 32) load_list<TAIL>(a, row, list);
     if (TAIL)
-        for (int i = tid; i < a.bitmap_words; i += kThreads) bitmap[i] = 0;
+        for (int i = tid; i < a.map_words / 4; i += kThreads) reinterpret_cast<uint4*>(map)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     if (!list.bad && (TAIL ? !list.any : list.mass == 0.0)) {
         // no teacher in this row: nothing is read (the whole cluster leaves here)
@@ -286,9 +303,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_topk_kernel(const Distill
     }
     if (TAIL) repeats = __syncthreads_or(repeats);
 
-    const float edge = edge_element(span);
-    stream_chunks<T, kThreads, kUnroll>(span, 0, chunks_of<T, kThreads, kUnroll>(span),
-                                        [&](uint4 (&v)[kUnroll], int first) { pass.take(v, first); });
+    stream_chunks<T, kThreads, kUnroll>(span, ahead, [&](uint4 (&v)[kUnroll], int it) { pass.take(v, it); });
     pass.take_edges(edge);
     SoftmaxRecord rec = cta_record<kThreads>(pass.rec, warp_records, pass.k2);
     cluster_wait_acquire();
@@ -341,12 +356,12 @@ struct DistillBwdArgs {
 };
 
 template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(kThreads, 6) distill_topk_bwd_kernel(const DistillBwdArgs a) {
+__global__ void __launch_bounds__(kBwdThreads, 6) distill_topk_bwd_kernel(const DistillBwdArgs a) {
     __shared__ int column[kMaxList];
     const int64_t row = blockIdx.x / a.pieces;
     const int piece = static_cast<int>(blockIdx.x % a.pieces);
     const int tid = threadIdx.x;
-    const RowMap<T, kThreads, kUnroll, VECTOR> map(static_cast<const T*>(a.logits) + row * a.ld,
+    const RowMap<T, kBwdThreads, kUnroll, VECTOR> map(static_cast<const T*>(a.logits) + row * a.ld,
                                                    static_cast<T*>(a.dlogits) + row * a.out_ld, a.cols, piece, a.chunks);
     const float* s = a.stats + row * kStats;
     const float all_m = s[0], all_log = s[1], tail_m = s[2], tail_log = s[3], log_norm = s[4], rest = s[5];
@@ -424,7 +439,8 @@ int forward(const void* logits, int64_t ld, const int64_t* index, const float* t
     DeviceContext ctx;
     rc = current_device_context(&ctx);
     if (rc != CREDIT_OK) return rc;
-    if (cluster == 0) cluster = row_split(rows, cols, ctx.sm_count);
+    const bool asked = cluster != 0;
+    if (!asked) cluster = row_split(rows, cols, 8 * ctx.sm_count, 4096);
     DistillArgs a;
     a.logits = logits;
     a.ld = ld;
@@ -438,11 +454,17 @@ int forward(const void* logits, int64_t ld, const int64_t* index, const float* t
     a.status = ctx.status;
     void* args[] = {&a};
     a.slice = row_slice(cols, cluster);
-    if (tail != 0 && a.slice > (1 << 20)) {   // the bitmap of a slice: at most 128 KiB
-        cluster = cluster < 4 ? 4 : cluster;
-        a.slice = row_slice(cols, cluster);
+    const int vec = dtype == CREDIT_BF16 ? 8 : 4;
+    if (tail != 0) {   // the map of a slice: at most 128 KiB
+        while (map_words(a.slice, vec) > 32 * 1024 + 4) {
+            if (asked)
+                return report_error(CREDIT_ERR_UNSUPPORTED, "cols=%lld: with a tail a row this wide needs a larger cluster than %d",
+                                    static_cast<long long>(cols), cluster);
+            cluster *= 2;
+            a.slice = row_slice(cols, cluster);
+        }
     }
-    a.bitmap_words = tail != 0 ? (a.slice + 31) / 32 : 0;
+    a.map_words = tail != 0 ? map_words(a.slice, vec) : 0;
     const void* func;
     if (dtype == CREDIT_BF16)
         func = tail ? reinterpret_cast<const void*>(&distill_topk_kernel<__nv_bfloat16, true>)
@@ -452,7 +474,7 @@ int forward(const void* logits, int64_t ld, const int64_t* index, const float* t
                     : reinterpret_cast<const void*>(&distill_topk_kernel<float, false>);
     rc = prepare_kernel(ctx, func);
     if (rc != CREDIT_OK) return rc;
-    return launch_kernel(func, rows * cluster, kThreads, cluster, a.bitmap_words * 4, stream, args);
+    return launch_kernel(func, rows * cluster, kThreads, cluster, a.map_words * 4, stream, args);
 }
 
 int backward(const void* logits, int64_t ld, const int64_t* index, const float* teacher, int top_k, const float* stats,
@@ -486,7 +508,7 @@ int backward(const void* logits, int64_t ld, const int64_t* index, const float* 
     a.inv_t = 1.0f / temperature;
     a.status = ctx.status;
     const bool vector = same_phase(logits, ld, dlogits, out_ld, rows, dtype);
-    const int chunk = kThreads * kUnroll * (dtype == CREDIT_BF16 ? 8 : 4);
+    const int chunk = kBwdThreads * kUnroll * (dtype == CREDIT_BF16 ? 8 : 4);
     a.chunks = chunks_per_piece(rows, cols, chunk, 4, ctx.sm_count);   // 1, 2, 4, 8: 239, 190, 175, 184 us at 2048 x 131072 bf16
     a.pieces = static_cast<int>((cols + static_cast<int64_t>(chunk) * a.chunks - 1) / (static_cast<int64_t>(chunk) * a.chunks));
     const void* func;
@@ -499,7 +521,7 @@ int backward(const void* logits, int64_t ld, const int64_t* index, const float* 
     rc = prepare_kernel(ctx, func);
     if (rc != CREDIT_OK) return rc;
     void* args[] = {&a};
-    return launch_kernel(func, rows * a.pieces, kThreads, 1, 0, stream, args);
+    return launch_kernel(func, rows * a.pieces, kBwdThreads, 1, 0, stream, args);
 }
 
 }  // namespace

@@ -110,21 +110,22 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
             return;
         }
     }
+    const int start = static_cast<int>(rank) * a.slice;
+    const RowSpan<T> span(x, start, max(0, min(a.slice, a.cols - start)));
+    uint4 ahead[kUnroll];
+    fetch_chunk<T, kThreads, kUnroll>(span, 0, ahead);
+    const float edge = edge_element(span);
     cluster_arrive_release();   // "this CTA runs": its shared memory may be written from now on
     const float picked = rank == 0 && tid == 0 ? target_logit(a, x, target) : 0.0f;
     if (TOP && tid == 0) init_top_buffer(t);
 
-    const int start = static_cast<int>(rank) * a.slice;
-    const int local = max(0, min(a.slice, a.cols - start));
-    const RowSpan<T> span(x, start, local);
     const float k2 = a.inv_t * kLog2e;
-    const float edge = edge_element(span);
     SoftmaxRecord rec = empty_record();
     const int chunks = chunks_of<T, kThreads, kUnroll>(span);
     TopCollector<T, kUnroll> collector(t, a.top_k, chunks);
-    stream_chunks<T, kThreads, kUnroll>(span, 0, chunks, [&](const uint4 (&v)[kUnroll], int first) {
+    stream_chunks<T, kThreads, kUnroll>(span, ahead, [&](const uint4 (&v)[kUnroll], int it) {
         const float top = chunk_max<T>(v);
-        if (TOP) collector.add(top, first / (kThreads * kUnroll));
+        if (TOP) collector.add(top, it);
         accumulate<T, kUnroll, ENTROPY>(v, top, k2, rec);
     });
     if (span.edges > 0) {
@@ -273,7 +274,8 @@ int forward(const void* logits, int64_t ld, const int64_t* targets, float* logpr
     DeviceContext ctx;
     rc = current_device_context(&ctx);
     if (rc != CREDIT_OK) return rc;
-    if (cluster == 0) cluster = row_split(rows, cols, ctx.sm_count);
+    // four CTAs an SM fit, and a few rows more than that still gain; choosing alternatives takes them longer together
+    if (cluster == 0) cluster = row_split(rows, cols, (top_k > 0 ? 30 : 41) * ctx.sm_count / 10, 8192);
     LogprobArgs a;
     a.logits = logits;
     a.ld = ld;

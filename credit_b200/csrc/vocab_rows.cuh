@@ -175,33 +175,35 @@ __device__ __forceinline__ int chunks_of(const RowSpan<T>& s) {
     return (s.nvec + THREADS * U - 1) / (THREADS * U);
 }
 
-// Calls f(v, first) for chunks [from, to) of U vectors a thread (vector first + u * THREADS is v[u];
-// places past the end hold -inf). Every thread of the CTA makes the same calls, so f may synchronise. The
-// next chunk is in flight while f runs.
-template <typename T, int THREADS, int U, typename F>
-__device__ __forceinline__ void stream_chunks(const RowSpan<T>& s, int from, int to, F&& f) {
-    constexpr int kPerChunk = THREADS * U;
+// A row in chunks of U vectors a thread: v[u] of chunk `it` is vector (it * U + u) * THREADS + threadIdx.x, places
+// past the end hold -inf. stream_chunks calls f(v, it) for every chunk, with the next one in flight; the first one
+// is fetched by the caller, before it sets anything else up.
+template <typename T, int THREADS, int U>
+__device__ __forceinline__ void fetch_chunk(const RowSpan<T>& s, int it, uint4 (&v)[U]) {
     const uint4* base = s.vectors();
-    auto fetch = [&](int it, uint4 (&v)[U]) {
-        const int i0 = it * kPerChunk + static_cast<int>(threadIdx.x);
-        if ((it + 1) * kPerChunk <= s.nvec) {
+    const int i0 = it * THREADS * U + static_cast<int>(threadIdx.x);
+    if ((it + 1) * THREADS * U <= s.nvec) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = load_stream(base + i0 + u * THREADS);
-        } else {
+        for (int u = 0; u < U; ++u) v[u] = load_stream(base + i0 + u * THREADS);
+    } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-                v[u] = i0 + u * THREADS < s.nvec ? load_stream(base + i0 + u * THREADS) : masked_vec<T>();
-        }
-    };
-    uint4 a[U], b[U];
-    if (from < to) fetch(from, a);
+        for (int u = 0; u < U; ++u)
+            v[u] = i0 + u * THREADS < s.nvec ? load_stream(base + i0 + u * THREADS) : masked_vec<T>();
+    }
+}
+
+template <typename T, int THREADS, int U, typename F>
+__device__ __forceinline__ void stream_chunks(const RowSpan<T>& s, uint4 (&a)[U], F&& f) {
+    constexpr int kPerChunk = THREADS * U;
+    const int chunks = chunks_of<T, THREADS, U>(s);
+    uint4 b[U];
 #pragma unroll 1
-    for (int it = from; it < to; it += 2) {
-        if (it + 1 < to) fetch(it + 1, b);
-        f(a, it * kPerChunk + static_cast<int>(threadIdx.x));
-        if (it + 1 >= to) break;
-        if (it + 2 < to) fetch(it + 2, a);
-        f(b, (it + 1) * kPerChunk + static_cast<int>(threadIdx.x));
+    for (int it = 0; it < chunks; it += 2) {
+        if (it + 1 < chunks) fetch_chunk<T, THREADS, U>(s, it + 1, b);
+        f(a, it);
+        if (it + 1 >= chunks) break;
+        if (it + 2 < chunks) fetch_chunk<T, THREADS, U>(s, it + 2, a);
+        f(b, it + 1);
     }
 }
 
@@ -246,14 +248,8 @@ struct RowMap {
     }
 
     // The piece's first chunk, on its way while the caller sets up; `run` takes it.
-    __device__ __forceinline__ void fetch(int it, uint4 (&v)[U]) const {
-        const int i0 = it * kVecs + static_cast<int>(threadIdx.x);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            v[u] = i0 + u * THREADS < span.nvec ? load_stream(span.vectors() + i0 + u * THREADS) : masked_vec<T>();
-    }
     __device__ __forceinline__ void first_chunk(uint4 (&v)[U]) const {
-        if (VECTOR) fetch(piece * chunks, v);
+        if (VECTOR) fetch_chunk<T, THREADS, U>(span, piece * chunks, v);
     }
 
     template <typename F>
@@ -277,7 +273,7 @@ struct RowMap {
             return;
         }
         for (int it = from; it < to; ++it) {
-            if (it > from) fetch(it, v);
+            if (it > from) fetch_chunk<T, THREADS, U>(span, it, v);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float y[E];
