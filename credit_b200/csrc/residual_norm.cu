@@ -242,22 +242,23 @@ struct RowWalk {
 #pragma unroll
         for (int k = 0; k < IN; ++k) places[k] = reinterpret_cast<const T*>(stage(at.stage) + k * a.slot_bytes);
         if (PATCH) {
-            bool patched = false;
 #pragma unroll
-            for (int k = 0; k < IN; ++k) {
-                if (in[k] == nullptr) continue;
-                const SliceSource<T> s = source(in[k], step);
-                places[k] += s.shift;
-                if (!s.complete(local)) {
-                    s.patch(stage(at.stage) + k * a.slot_bytes, local);
-                    patched = true;
-                }
-            }
-            if (patched) {   // the same in every thread
-                fence_proxy_async_smem();   // a later copy into this stage follows these stores
-                __syncthreads();
-            }
+            for (int k = 0; k < IN; ++k)
+                places[k] += (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(in[k])) + static_cast<uint32_t>(offset(step)) * sizeof(T)) %
+                             16u / sizeof(T);
+            // only a slice at the very start or end of the matrix can lack elements
+            if (offset(step) < 16 || offset(step) + local + 16 > matrix) patch(in, at.stage, step);
         }
+    }
+    __device__ __forceinline__ void patch(const void* const (&in)[IN], int i, int step) const {
+#pragma unroll
+        for (int k = 0; k < IN; ++k)
+            if (in[k] != nullptr) {
+                const SliceSource<T> s = source(in[k], step);
+                if (!s.complete(local)) s.patch(stage(i) + k * a.slot_bytes, local);
+            }
+        fence_proxy_async_smem();   // a later copy into this stage follows these stores
+        __syncthreads();
     }
     // by warp 0
     __device__ __forceinline__ void fill(const void* const (&in)[IN], int i, int step) const {
