@@ -52,6 +52,9 @@ def main(argv: list[str]) -> int:
         if name == "layernorm_backward_stats":
             need = L.layernorm_backward_stats_workspace_bytes(rows, cols, spec.dtype)
             kw["workspace"] = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        if name == "residual_norm_backward":
+            need = L.residual_norm_backward_workspace_bytes(rows, cols, spec.dtype, cluster)
+            kw["workspace"] = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
 
         def call():
             L.NATIVE_LAUNCHERS[name](ins, outs, cluster, dict(opts), **kw)

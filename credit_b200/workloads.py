@@ -13,6 +13,7 @@ same call on the CPU always gives the same bits.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 from typing import Callable
 
@@ -175,6 +176,87 @@ def make_quant_inputs(rows: int, cols: int, device, seed: int = 0) -> TensorTupl
     return (_uniform((rows, cols), -1.0, 1.0, device, _generator(device, seed)),)
 
 
+# The end of a decoder: bf16 matrices, fp32 parameters and row scalars.
+def make_residual_norm_inputs(rows: int, cols: int, device, seed: int = 0,
+                              dtype: torch.dtype = torch.bfloat16) -> TensorTuple:
+    """(block, residual, post_weight, gate, pre_weight): matrices ~ N(0,1) rounded to `dtype`, parameters ~ U(0.5, 1.5)."""
+    gen = _generator(device, seed)
+    block, residual = (_normal((rows, cols), 0.0, 1.0, device, gen).to(dtype) for _ in range(2))
+    return (block, residual, *(_uniform((cols,), 0.5, 1.5, device, gen) for _ in range(3)))
+
+
+def make_residual_norm_backward_inputs(rows: int, cols: int, device, seed: int = 0,
+                                       dtype: torch.dtype = torch.bfloat16, eps: float = 1.0e-6) -> TensorTuple:
+    """(dy, dresidual_out, block, residual_out, post_weight, gate, pre_weight, post_rstd, pre_rstd)."""
+    block, residual_out, post_weight, gate, pre_weight = make_residual_norm_inputs(rows, cols, device, seed, dtype)
+    gen = _generator(device, seed + 1)
+    dy, dresidual_out = (_normal((rows, cols), 0.0, 1.0, device, gen).to(dtype) for _ in range(2))
+    post_rstd, pre_rstd = (torch.rsqrt(t.float().square().mean(dim=-1) + eps) for t in (block, residual_out))
+    return dy, dresidual_out, block, residual_out, post_weight, gate, pre_weight, post_rstd, pre_rstd
+
+
+def make_token_logprobs_inputs(rows: int, cols: int, device, seed: int = 0,
+                               dtype: torch.dtype = torch.bfloat16) -> TensorTuple:
+    """(logits, targets): logits ~ N(0, 2.5) with one planted likely token a row, the targets."""
+    gen = _generator(device, seed)
+    logits = _normal((rows, cols), 0.0, 2.5, device, gen)
+    targets = torch.randint(0, cols, (rows,), device=device, generator=gen)
+    logits[torch.arange(rows, device=device), targets] = 12.0
+    return logits.to(dtype), targets
+
+
+def make_token_logprobs_backward_inputs(rows: int, cols: int, device, seed: int = 0,
+                                        dtype: torch.dtype = torch.bfloat16) -> TensorTuple:
+    """(logits, targets, stats, entropy, dlogprob, dentropy), stats and entropy as a forward call saves them."""
+    logits, targets = make_token_logprobs_inputs(rows, cols, device, seed, dtype)
+    gen = _generator(device, seed + 1)
+    stats, entropy = (torch.empty(rows, n, device=device, dtype=torch.float32) for n in (2, 1))
+    step = max(1, (1 << 26) // max(cols, 1))
+    for r0 in range(0, rows, step):
+        x = logits[r0:r0 + step].float()
+        top = x.amax(dim=-1)
+        log_p = torch.log_softmax(x, dim=-1)
+        stats[r0:r0 + step, 0] = top
+        stats[r0:r0 + step, 1] = torch.logsumexp(x, dim=-1) - top
+        entropy[r0:r0 + step, 0] = -(log_p.exp() * log_p).sum(dim=-1)
+    return (logits, targets, stats, entropy[:, 0].contiguous(), _normal((rows,), 0.0, 1.0, device, gen),
+            _uniform((rows,), 0.0, 0.01, device, gen))
+
+
+DISTILL_LIST = 64      # teacher columns a row in the registry's inputs
+
+
+def make_distill_topk_inputs(rows: int, cols: int, device, seed: int = 0,
+                             dtype: torch.dtype = torch.bfloat16) -> TensorTuple:
+    """(logits, teacher_index, teacher_logprob): distinct columns, 0.9 of the teacher's mass in the list."""
+    logits, _ = make_token_logprobs_inputs(rows, cols, device, seed, dtype)
+    gen = _generator(device, seed + 1)
+    k = min(DISTILL_LIST, cols)
+    stride = cols // k
+    index = torch.arange(k, device=device) * stride + torch.randint(0, stride, (rows, k), device=device, generator=gen)
+    value = torch.log_softmax(_normal((rows, k), 0.0, 2.0, device, gen), dim=-1)
+    return logits, index, value + math.log(0.9)
+
+
+def make_distill_topk_backward_inputs(rows: int, cols: int, device, seed: int = 0,
+                                      dtype: torch.dtype = torch.bfloat16) -> TensorTuple:
+    """(logits, teacher_index, teacher_logprob, stats, dloss), stats as a forward call with a tail saves them."""
+    logits, index, value = make_distill_topk_inputs(rows, cols, device, seed, dtype)
+    stats = torch.empty(rows, 6, device=device, dtype=torch.float32)
+    step = max(1, (1 << 26) // max(cols, 1))
+    for r0 in range(0, rows, step):
+        x = logits[r0:r0 + step].float()
+        for c in (0, 2):      # all columns, then those outside the list
+            top = x.amax(dim=-1)
+            stats[r0:r0 + step, c] = top
+            stats[r0:r0 + step, c + 1] = torch.logsumexp(x - top[:, None], dim=-1)
+            x.scatter_(1, index[r0:r0 + step], -math.inf)
+    stats[:, 4] = 0.0
+    stats[:, 5] = 1.0 - value.exp().sum(dim=-1)
+    dloss = _uniform((rows,), 0.5, 1.5, device, _generator(device, seed + 2))
+    return logits, index, value, stats, dloss
+
+
 def ffn_flops(rows: int, cols: int, hidden: int) -> int:
     return 2 * (2 * rows * cols * hidden)
 
@@ -268,6 +350,48 @@ WORKLOADS: dict[str, WorkloadSpec] = {
         modeled_bytes_per_element=9.0, reread_bytes_per_element=4.0, staged_bytes_per_element=4,
         reductions_per_stage=(1,), atol=1.0e-6, rtol=1.0e-6,
         algorithmic_bytes=lambda r, c: r * c * 5 + r * 4,
+    ),
+    "residual_norm_forward": WorkloadSpec(
+        name="residual_norm_forward", label="Post norm, gate, residual and pre norm forward", category="normalization",
+        rows=16384, cols=8192, dtype=torch.bfloat16, input_factory=make_residual_norm_inputs, eps=1.0e-6,
+        modeled_bytes_per_element=12.0, reread_bytes_per_element=4.0, staged_bytes_per_element=4,
+        reductions_per_stage=(1, 1), atol=2.0e-2, rtol=2.0e-2,
+        algorithmic_bytes=lambda r, c: 4 * r * c * 2 + 3 * c * 4 + 2 * r * 4,
+    ),
+    "residual_norm_backward": WorkloadSpec(
+        name="residual_norm_backward", label="Post norm, gate, residual and pre norm backward", category="normalization",
+        rows=16384, cols=4096, dtype=torch.bfloat16, input_factory=make_residual_norm_backward_inputs, eps=1.0e-6,
+        modeled_bytes_per_element=20.0, reread_bytes_per_element=8.0, staged_bytes_per_element=8,
+        reductions_per_stage=(4,), atol=2.0e-2, rtol=2.0e-2,
+        algorithmic_bytes=lambda r, c: 6 * r * c * 2 + 6 * c * 4 + 2 * r * 4,
+    ),
+    "token_logprobs_forward": WorkloadSpec(
+        name="token_logprobs_forward", label="Token log probabilities and entropy", category="softmax",
+        rows=4096, cols=131072, dtype=torch.bfloat16, input_factory=make_token_logprobs_inputs, eps=0.0,
+        modeled_bytes_per_element=4.0, reread_bytes_per_element=2.0, staged_bytes_per_element=0,
+        reductions_per_stage=(3,), atol=1.0e-4, rtol=1.0e-5,
+        algorithmic_bytes=lambda r, c: r * c * 2 + r * (8 + 4 + 8 + 4),
+    ),
+    "token_logprobs_backward": WorkloadSpec(
+        name="token_logprobs_backward", label="Token log probabilities backward", category="softmax",
+        rows=4096, cols=65536, dtype=torch.bfloat16, input_factory=make_token_logprobs_backward_inputs, eps=0.0,
+        modeled_bytes_per_element=4.0, reread_bytes_per_element=0.0, staged_bytes_per_element=0,
+        reductions_per_stage=(), atol=2.0e-2, rtol=2.0e-2,
+        algorithmic_bytes=lambda r, c: 2 * r * c * 2 + r * 28,
+    ),
+    "distill_topk_forward": WorkloadSpec(
+        name="distill_topk_forward", label="Distillation from a teacher's top logits", category="softmax",
+        rows=2048, cols=131072, dtype=torch.bfloat16, input_factory=make_distill_topk_inputs, eps=0.0,
+        modeled_bytes_per_element=4.0, reread_bytes_per_element=2.0, staged_bytes_per_element=0,
+        reductions_per_stage=(3,), atol=1.0e-4, rtol=1.0e-5,
+        algorithmic_bytes=lambda r, c: r * c * 2 + r * (12 * min(DISTILL_LIST, c) + 28),
+    ),
+    "distill_topk_backward": WorkloadSpec(
+        name="distill_topk_backward", label="Distillation from a teacher's top logits backward", category="softmax",
+        rows=2048, cols=131072, dtype=torch.bfloat16, input_factory=make_distill_topk_backward_inputs, eps=0.0,
+        modeled_bytes_per_element=4.0, reread_bytes_per_element=0.0, staged_bytes_per_element=0,
+        reductions_per_stage=(), atol=2.0e-2, rtol=2.0e-2,
+        algorithmic_bytes=lambda r, c: 2 * r * c * 2 + r * (12 * min(DISTILL_LIST, c) + 28),
     ),
 }
 
