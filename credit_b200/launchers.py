@@ -513,9 +513,12 @@ def allocate_outputs(name: str, inputs: tuple[torch.Tensor, ...], top_k: int = 0
     if name == "distill_topk_forward":
         return (fp32(rows), fp32(rows, 6))
     if name in ("token_logprobs_backward", "distill_topk_backward"):
-        # rows as far apart as the logits': both then start at the same place between 16-byte boundaries
-        stride = max(int(x.stride(0)), cols)
-        return (torch.empty((rows, stride), device=dev, dtype=x.dtype)[:, :cols],)
+        # rows that start at the same place between two 16-byte boundaries as the logits' do, without their padding
+        vec = 16 // x.element_size()
+        stride = cols + (max(int(x.stride(0)), cols) - cols) % vec
+        shift = x.data_ptr() % 16 // x.element_size()
+        flat = torch.empty(shift + rows * stride, device=dev, dtype=x.dtype)
+        return (flat[shift:].view(rows, stride)[:, :cols],)
     if name == "row_reduce":
         return (
             torch.empty(rows, device=dev, dtype=torch.float32),

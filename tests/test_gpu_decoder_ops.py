@@ -274,10 +274,9 @@ def _run_logprobs(x, targets, top_k=0, temperature=1.0, cluster=0, ld=None, shif
     return outs
 
 
-# the last two: more rows than twice the SMs, several rows for each persistent CTA
 LOGIT_SHAPES = [(1, 1, None, 0), (3, 2, None, 0), (2, 7, 9, 3), (5, 255, None, 1), (4, 257, 320, 0), (3, 1000, 1024, 8),
                 (2, 4099, None, 5), (3, 8192, None, 0), (2, 8200, 8260, 1), (2, 50001, None, 0), (2, 131072, None, 0),
-                (1, 262147, 262400, 7), (300, 520, None, 0), (700, 8200, None, 0), (310, 16411, 16500, 3)]
+                (1, 262147, 262400, 7), (300, 520, None, 0)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -336,7 +335,7 @@ def test_top_alternatives_of_sorted_and_constant_wide_rows(native_lib, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 def test_many_rows_with_masks_and_special_values(native_lib, dtype):
-    """The persistent form: rows of every kind next to one another in one CTA's walk."""
+    """More rows than are resident at once, of every kind next to one another."""
     rows, cols = 900, 9001
     x, targets = _logits(rows, cols, dtype, 50)
     x[1::9] = -math.inf
@@ -532,7 +531,7 @@ def test_distill_lists_and_masks(native_lib, dtype, tail, cluster):
 
 @pytest.mark.parametrize("tail", [True, False])
 def test_distill_many_rows(native_lib, tail):
-    """The persistent form: lists and masks of every kind next to one another in one CTA's walk."""
+    """Rows that one CTA each takes, lists and masks of every kind next to one another."""
     rows, cols, k = 700, 9001, 8
     x, _ = _logits(rows, cols, torch.bfloat16, 51)
     index, logprob = _teacher(x, k, 52)
@@ -728,3 +727,102 @@ def test_bytes_around_the_logits_stay(native_lib):
         _launch("distill_topk_backward", (logits, index.to(DEV), logprob.to(DEV), saved.float().to(DEV),
                                           torch.ones(rows, device=DEV)), (out,))
         assert bool((buffer[0] == 7).all()) and bool((buffer[-1] == 7).all()) and bool((buffer[:, cols:] == 7).all())
+
+
+def test_gradient_buffers_take_the_vector_form_without_the_padding(native_lib):
+    """allocate_outputs: the logits' alignment, not their row stride."""
+    for dtype in TYPES:
+        wide = torch.zeros(6, 5000, device=DEV, dtype=dtype)
+        for view in (wide[:, :1000], wide[:, 3:1003], wide[:, :999], wide[1:2, 7:8], wide[:0, :40], wide):
+            (out,) = L.allocate_outputs("token_logprobs_backward", (view,))
+            vec = 16 // view.element_size()
+            assert out.shape == view.shape and out.dtype == dtype
+            if view.shape[0] > 1:
+                assert (out.data_ptr() - view.data_ptr()) % 16 == 0 and (out.stride(0) - view.stride(0)) % vec == 0
+                assert out.stride(0) < view.shape[1] + vec
+    x, targets = _logits(6, 1000, torch.bfloat16, 60)
+    wide = torch.zeros(6, 5000, device=DEV, dtype=torch.bfloat16)
+    logits = wide[:, 3:1003]
+    logits.copy_(x)
+    _, stats, _, _, _ = D.token_logprobs_forward(x, targets)
+    ins = (logits, targets.to(DEV), stats.float().to(DEV), None, torch.ones(6, device=DEV), None)
+    (out,) = L.allocate_outputs("token_logprobs_backward", ins)
+    _launch("token_logprobs_backward", ins, (out,))
+    want, mag, logp = D.token_logprobs_backward(x, targets, stats.float(), None, torch.ones(6))
+    _within(out, want, mag * U * (64 + 16 * logp.abs() + 8 * 20) + _rounding(torch.bfloat16, want), "dlogits")
+
+
+def test_launchers_refuse(native_lib):
+    x, targets = _logits(4, 600, torch.float32, 61)
+    logits, targets = x.to(DEV), targets.to(DEV)
+    outs = L.allocate_outputs("token_logprobs_forward", (logits, targets), top_k=4)
+    index, value = (t.to(DEV) for t in _teacher(x, 6, 62))
+    kd = L.allocate_outputs("distill_topk_forward", (logits,))
+    f32 = torch.zeros(4, device=DEV)
+
+    def bad(name, inputs, outputs, match, **kw):
+        with pytest.raises((ValueError, N.CreditError), match=match):
+            L.NATIVE_LAUNCHERS[name](inputs, outputs, **kw)
+
+    bad("token_logprobs_forward", (logits.half(), targets), outs, "dtype")
+    bad("token_logprobs_forward", (logits.T, targets), outs, "contiguous rows")
+    bad("token_logprobs_forward", (logits[:1].expand(4, 600), targets), outs, "contiguous rows")
+    bad("token_logprobs_forward", (logits[0], targets), outs, "two dimensions")
+    bad("token_logprobs_forward", (logits, targets.int()), outs, "targets must have dtype")
+    bad("token_logprobs_forward", (logits, targets[:3]), outs, "targets must have shape")
+    bad("token_logprobs_forward", (logits, targets.cpu()), outs, "targets must be a CUDA tensor")
+    bad("token_logprobs_forward", (logits, None), outs, "go together")
+    bad("token_logprobs_forward", (logits, targets), (*outs[:3], None, outs[4]), "go together")
+    bad("token_logprobs_forward", (logits, targets), outs, "temperature", temperature=0.0)
+    bad("token_logprobs_forward", (logits, targets), outs, "cluster_size", cluster_size=5)
+    wide = torch.zeros(4, 129, device=DEV)
+    bad("token_logprobs_forward", (logits, targets), (*outs[:3], wide, wide.long()), "top_k")
+    bad("token_logprobs_backward", (logits, targets, outs[1], None, f32, f32), (torch.empty_like(logits),), "entropy")
+    shifted = torch.zeros(4 * 600 + 1, device=DEV)
+    bad("token_logprobs_backward", (shifted[:-1].view(4, 600), targets, outs[1], None, f32, None),
+        (shifted[1:].view(4, 600),), "overlap")
+    bad("distill_topk_forward", (logits, index[:, :5], value), kd, "teacher_index must be contiguous")
+    bad("distill_topk_forward", (logits, index, value.double()), kd, "teacher_logprob must have dtype")
+    bad("distill_topk_forward", (logits, index, value), (kd[0], kd[1][:, :5].contiguous()), "stats must have shape")
+    norm = tuple(_on_gpu(t) for t in _norm_inputs(4, 512, torch.float32, 63))
+    outs = L.allocate_outputs("residual_norm_forward", norm)
+    bad("residual_norm_forward", (norm[0], norm[1].bfloat16(), *norm[2:]), outs, "residual must have dtype")
+    bad("residual_norm_forward", (*norm[:2], None, *norm[3:]), outs, "go together")
+    bad("residual_norm_forward", norm, (outs[0], outs[0], *outs[2:]), "differ")
+    bad("residual_norm_forward", norm, outs, "eps", eps=0.0)
+    back = (norm[0], None, norm[0], outs[0], *norm[2:], outs[2], outs[3])
+    grads = L.allocate_outputs("residual_norm_backward", back)
+    bad("residual_norm_backward", back, grads, "workspace", workspace=torch.empty(64, dtype=torch.uint8, device=DEV))
+    bad("residual_norm_backward", back, (*grads[:3], None, grads[4]), "go together")
+    assert N.device_status() == 0
+
+
+def test_one_value_more_than_32_bits_of_elements(native_lib):
+    """Offsets past 2^31 elements: the last rows of a matrix of 2.2e9 logits, and of one as wide of the norms."""
+    rows, cols = 17000, 131072
+    buffer = torch.empty(rows, cols, device=DEV, dtype=torch.bfloat16)
+    x, targets = _logits(2, cols, torch.bfloat16, 64)
+    buffer[-2:] = x.to(DEV)
+    target = torch.full((rows,), -1, device=DEV)
+    target[-2:] = targets.to(DEV)
+    outs = L.allocate_outputs("token_logprobs_forward", (buffer, target), top_k=3)
+    _launch("token_logprobs_forward", (buffer, target), outs)
+    _check_logprobs(x, targets, [o[-2:] for o in outs], 1.0, 3)
+    g = torch.ones(rows, device=DEV)
+    _launch("token_logprobs_backward", (buffer, target, outs[1], None, g, None), (buffer,))     # in place
+    _, stats, _, _, _ = D.token_logprobs_forward(x, targets)
+    want, mag, logp = D.token_logprobs_backward(x, targets, outs[1][-2:].cpu(), None, torch.ones(2))
+    _within(buffer[-2:], want, mag * U * (64 + 16 * logp.abs() + 8 * 20) + _rounding(torch.bfloat16, want), "dlogits")
+    assert float(buffer[:-2].abs().max()) == 0.0
+    del buffer
+    rows, cols = 540000, 4096
+    block = torch.zeros(rows, cols, device=DEV, dtype=torch.bfloat16)
+    last = _norm_inputs(2, cols, torch.bfloat16, 65)
+    block[-2:] = last[0].to(DEV)
+    residual = torch.zeros_like(block)
+    residual[-2:] = last[1].to(DEV)
+    ins = (block, residual, *(t.to(DEV) for t in last[2:]))
+    outs = L.allocate_outputs("residual_norm_forward", ins)
+    _launch("residual_norm_forward", ins, outs, residual_scale=0.7, eps=1e-5)
+    _check_norm_forward(last, [o[-2:] for o in outs], 0.7, 1e-5, torch.bfloat16)
+    assert N.device_status() == 0
