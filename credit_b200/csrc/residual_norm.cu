@@ -106,6 +106,9 @@ template <typename T, int W>
 __device__ __forceinline__ void store_elems(T* p, const float (&x)[W]) {
     if constexpr (W == 1) {
         Vec<T>::store(p, x[0]);
+    } else if constexpr (W * sizeof(T) == 32) {
+        __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
+        __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(x[4], x[5], x[6], x[7]));
     } else {
         __stcs(reinterpret_cast<uint4*>(p), Vec<T>::pack(x));
     }
@@ -559,16 +562,15 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_bwd_kern
         last = at.stage;
         at.advance(a.ring.stages);
     }
-    float* mine = a.partials + static_cast<size_t>(walk.cluster) * 2 * a.ring.cols + walk.start;
+    // the finishing kernel may be set up while these are written; it waits for this grid's end
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    float* sums_out = a.partials + static_cast<size_t>(walk.cluster) * 2 * a.ring.cols + walk.start;
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int e = e0 + u * kStride;
         if (e < local) {
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                mine[e + j] = col_c[u][j];
-                mine[a.ring.cols + e + j] = col_w[u][j];
-            }
+            store_elems<float, W>(sums_out + e, col_c[u]);
+            store_elems<float, W>(sums_out + a.ring.cols + e, col_w[u]);
         }
     }
     if (walk.nranks > 1) cluster_sync_all();   // no CTA leaves while a peer may still send to it
@@ -580,6 +582,7 @@ __global__ void __launch_bounds__(kFinishCols* kFinishStrands)
     residual_norm_finish_kernel(const float* partials, int clusters, int cols, const float* post_weight, const float* gate,
                                 float* dpost_weight, float* dgate, float* dpre_weight) {
     __shared__ float strand[2][kFinishStrands][kFinishCols];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x % kFinishCols, s = threadIdx.x / kFinishCols;
     const int c = blockIdx.x * kFinishCols + lane;
     float both[2] = {0.0f, 0.0f};
@@ -593,15 +596,16 @@ __global__ void __launch_bounds__(kFinishCols* kFinishStrands)
     strand[0][s][lane] = both[0];
     strand[1][s][lane] = both[1];
     __syncthreads();
-    if (s != 0 || c >= cols) return;
-    both[0] = both[1] = 0.0f;
-    for (int i = 0; i < kFinishStrands; ++i) {
-        both[0] += strand[0][i][lane];
-        both[1] += strand[1][i][lane];
+    if (s > 1 || c >= cols) return;
+    float sum = 0.0f;   // C in strand 0's warp, dpre_weight in strand 1's
+#pragma unroll
+    for (int i = 0; i < kFinishStrands; ++i) sum += strand[s][i][lane];
+    if (s == 1) {
+        dpre_weight[c] = sum;
+    } else {
+        if (dpost_weight != nullptr) dpost_weight[c] = gate != nullptr ? sum * gate[c] : sum;
+        if (dgate != nullptr) dgate[c] = post_weight != nullptr ? sum * post_weight[c] : sum;
     }
-    dpre_weight[c] = both[1];
-    if (dpost_weight != nullptr) dpost_weight[c] = gate != nullptr ? both[0] * gate[c] : both[0];
-    if (dgate != nullptr) dgate[c] = post_weight != nullptr ? both[0] * post_weight[c] : both[0];
 }
 
 // ---------------------------------------------------------------------------
@@ -807,9 +811,18 @@ int backward(const void* dy, const void* dresidual_out, const void* block, const
     void* args[] = {&a};
     rc = launch_kernel(p.func, static_cast<int64_t>(p.clusters) * p.cluster, p.threads, p.cluster, p.smem, stream, args);
     if (rc != CREDIT_OK) return rc;
-    residual_norm_finish_kernel<<<(p.ring.cols + kFinishCols - 1) / kFinishCols, kFinishCols * kFinishStrands, 0, s>>>(
-        a.partials, p.clusters, p.ring.cols, post_weight, gate, dpost_weight, dgate, dpre_weight);
-    const cudaError_t err = cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((p.ring.cols + kFinishCols - 1) / kFinishCols));
+    cfg.blockDim = dim3(kFinishCols * kFinishStrands);
+    cfg.stream = s;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    const float* partials = a.partials;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, residual_norm_finish_kernel, partials, p.clusters, p.ring.cols, post_weight,
+                                               gate, dpost_weight, dgate, dpre_weight);
     if (err != cudaSuccess) return report_error(CREDIT_ERR_CUDA, "column sums: %s", cudaGetErrorString(err));
     return CREDIT_OK;
 }
