@@ -150,7 +150,7 @@ __device__ __forceinline__ uint64_t keep_largest(TopBuffer& t, int n, int k) {
     return t.fill < k ? 0 : t.lowest;
 }
 
-// The same, sorted descending: with one key a thread at most, every key counts the larger ones, which is
+// The same, sorted descending: with one key a thread at most, the larger ones are counted for each, which is
 // its place; more go through the digits first. Returns the k-th (0 when there are fewer).
 __device__ __noinline__ uint64_t rank_largest(TopBuffer& t, int n, int k) {
     const int tid = threadIdx.x;
@@ -159,21 +159,24 @@ __device__ __noinline__ uint64_t rank_largest(TopBuffer& t, int n, int k) {
         n = t.fill;
         __syncthreads();
     }
-    const uint64_t mine = tid < n ? t.keys[tid] : 0;
+    // few keys: 4 or 2 neighbouring threads share one and count a part of the others each
+    const int shift = n <= kTopThreads / 4 ? 2 : (n <= kTopThreads / 2 ? 1 : 0), share = 1 << shift;
+    const int at = tid >> shift, part = tid & (share - 1);
+    const uint64_t mine = at < n ? t.keys[at] : 0;
     int place = 0;
     if (mine != 0) {
-        int i = 0;
-#pragma unroll 1
-        for (; i + 4 <= n; i += 4) {
+        int i = part * 2;
+#pragma unroll 2
+        for (; i + 2 <= n; i += 2 * share) {
             const ulonglong2 p = *reinterpret_cast<const ulonglong2*>(&t.keys[i]);
-            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(&t.keys[i + 2]);
-            place += (p.x > mine) + (p.y > mine) + (q.x > mine) + (q.y > mine);
+            place += (p.x > mine) + (p.y > mine);
         }
-#pragma unroll 1
-        for (; i < n; ++i) place += t.keys[i] > mine;
+        if (i < n) place += t.keys[i] > mine;
     }
-    const int kept = __syncthreads_count(mine != 0);
-    if (mine != 0 && place < k) t.keys[place] = mine;
+    if (share > 1) place += __shfl_xor_sync(0xffffffffu, place, 1);
+    if (share > 2) place += __shfl_xor_sync(0xffffffffu, place, 2);
+    const int kept = __syncthreads_count(mine != 0 && part == 0);
+    if (mine != 0 && part == 0 && place < k) t.keys[place] = mine;
     if (tid == 0) t.fill = min(kept, k);
     __syncthreads();
     return kept >= k ? t.keys[k - 1] : 0;
@@ -280,13 +283,16 @@ struct TopCollector {
         const float floor = image_value(least);   // NaN: only NaN reaches it
         const bool nan = floor != floor;
         const int groups = (chunks + per_group - 1) / max(per_group, 1);
-#pragma unroll 1
-        for (int g = 0; g < groups; ++g) {
-            const float x = t.group[g][tid];
-            if (nan ? x != x : !(x < floor)) {
-                const int at = atomicAdd(&t.notes, 1);
-                if (at < kTopCapacity) t.noted[at] = g * kTopThreads + tid;
-            }
+        uint32_t reach = 0;   // groups, a bit each
+#pragma unroll
+        for (int g = 0; g < kTopGroups; ++g) {
+            const float x = g < groups ? t.group[g][tid] : -CUDART_INF_F;
+            if (nan ? x != x : !(x < floor)) reach |= 1u << g;
+        }
+        if (reach != 0) {
+            int at = atomicAdd(&t.notes, __popc(reach));
+            for (; reach != 0; reach &= reach - 1, ++at)
+                if (at < kTopCapacity) t.noted[at] = (__ffs(reach) - 1) * kTopThreads + tid;
         }
         __syncthreads();
         const int notes = t.notes, vectors = U * per_group;
@@ -294,15 +300,24 @@ struct TopCollector {
         if (!overflow) {
 #pragma unroll 1
             for (int i = tid; i < notes * vectors; i += kTopThreads) {
-                const int note = t.noted[i / vectors], place = i % vectors;
+                const int which = per_group == 1 ? i / U : i / vectors, place = i - which * vectors, note = t.noted[which];
                 const int v = ((note / kTopThreads * per_group) * U + place) * kTopThreads + note % kTopThreads;
                 if (v >= span.nvec) continue;
-                const int column = span.vector_column(v);
                 float x[E];
                 Vec<T>::unpack(span.vectors()[v], x);
+                uint32_t hits = 0;
 #pragma unroll
                 for (int j = 0; j < E; ++j)
-                    if (nan ? x[j] != x[j] : !(x[j] < floor)) offer(x[j], column + j);
+                    if (nan ? x[j] != x[j] : !(x[j] < floor)) hits |= 1u << j;
+                if (hits == 0) continue;
+                int at = atomicAdd(&t.count, __popc(hits));
+                const int column = span.vector_column(v);
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    if (hits >> j & 1u) {
+                        if (at < kTopCapacity) t.keys[at] = element_key(x[j], column + j);
+                        ++at;
+                    }
             }
         }
         __syncthreads();
@@ -317,13 +332,21 @@ struct TopCollector {
     }
 };
 
+// Smallest 64-bit key over a warp.
+__device__ __forceinline__ uint64_t warp_min_key(uint64_t key) {
+    const uint32_t hi = static_cast<uint32_t>(key >> 32), lo = static_cast<uint32_t>(key);
+    const uint32_t m = __reduce_min_sync(0xffffffffu, hi);
+    const uint32_t l = __reduce_min_sync(0xffffffffu, hi == m ? lo : 0xffffffffu);
+    return (static_cast<uint64_t>(m) << 32) | l;
+}
+
 // Rank 0: the k largest of `lists` sorted lists of k keys (zeros at their ends) into t.keys[0, fill), sorted. Of
 // every list the first ceil(k / lists) entries are k together, so nothing below the smallest of those can
 // be among the k largest. All threads, behind a barrier.
 __device__ __forceinline__ void merge_lists(TopBuffer& t, const unsigned long long* gathered, int lists, int k) {
     const int share = (k + lists - 1) / lists - 1;
-    uint64_t floor = ~0ull;
-    for (int r = 0; r < lists; ++r) floor = min(floor, static_cast<uint64_t>(gathered[r * k + share]));
+    const int lane = threadIdx.x & 31;
+    const uint64_t floor = warp_min_key(lane < lists ? gathered[lane * k + share] : ~0ull);
     if (threadIdx.x == 0) t.count = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < lists * k; i += kTopThreads) {

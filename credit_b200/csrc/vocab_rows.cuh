@@ -194,7 +194,6 @@ __device__ __forceinline__ void fetch_chunk(const RowSpan<T>& s, int it, uint4 (
 
 template <typename T, int THREADS, int U, typename F>
 __device__ __forceinline__ void stream_chunks(const RowSpan<T>& s, uint4 (&a)[U], F&& f) {
-    constexpr int kPerChunk = THREADS * U;
     const int chunks = chunks_of<T, THREADS, U>(s);
     uint4 b[U];
 #pragma unroll 1
