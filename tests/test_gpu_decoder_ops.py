@@ -826,3 +826,74 @@ def test_one_value_more_than_32_bits_of_elements(native_lib):
     _launch("residual_norm_forward", ins, outs, residual_scale=0.7, eps=1e-5)
     _check_norm_forward(last, [o[-2:] for o in outs], 0.7, 1e-5, torch.bfloat16)
     assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(2, 1 << 22), (1, (1 << 22) - 5), (150000, 33)])
+def test_widest_and_most_rows(native_lib, dtype, rows, cols):
+    """The largest width, and more rows than two grid dimensions of 65535 would hold, against fp64 torch on the GPU.
+    Tolerances as in _check_logprobs and _check_logprob_gradient (512 additions a chain at the largest width)."""
+    gen = torch.Generator(device=DEV).manual_seed(71)
+    x = (torch.randn(rows, cols, generator=gen, device=DEV) * 2.0).to(dtype)
+    targets = torch.randint(0, cols, (rows,), generator=gen, device=DEV)
+    outs = _poisoned(L.allocate_outputs("token_logprobs_forward", (x, targets), top_k=5))
+    _launch("token_logprobs_forward", (x, targets), outs)
+    z = x.double()
+    logp = torch.log_softmax(z, -1)
+    log_n = math.log2(cols)
+    e_sum = (768 + 64 * log_n) * U
+    assert float((outs[0] - logp.gather(1, targets[:, None])[:, 0]).abs().max()) < e_sum + 8 * U * 40
+    entropy = -(logp.exp() * logp).sum(-1)
+    assert float((outs[2] - entropy).abs().max()) < e_sum * (2 + log_n) + 8 * U * log_n
+    value, index = torch.sort(x, dim=-1, descending=True, stable=True)
+    assert torch.equal(outs[4], index[:, :5])
+    del value, index
+    g = torch.rand(rows, generator=gen, device=DEV)
+    (grad,) = L.allocate_outputs("token_logprobs_backward", (x,))
+    _launch("token_logprobs_backward", (x, targets, outs[1], None, g, None), (grad,))
+    want = -logp.exp() * g[:, None].double()
+    want.scatter_add_(1, targets[:, None], g[:, None].double())
+    tol = (64 + 16 * 40 + 8 * 20) * U * logp.exp() + 768 * U * logp.exp() + 1e-37
+    tol.scatter_add_(1, targets[:, None], torch.full((rows, 1), (64 + 8 * 20) * U, device=DEV, dtype=torch.float64))
+    tol += want.abs() * (2.0 ** -8 if dtype == torch.bfloat16 else 0.0)
+    assert bool(((grad.double() - want).abs() <= tol).all())
+    del want, tol
+    k = 16
+    teacher = torch.arange(k, device=DEV) * (cols // k) + torch.randint(0, cols // k, (rows, k), generator=gen, device=DEV)
+    weight = torch.log_softmax(torch.randn(rows, k, generator=gen, device=DEV), -1) + math.log(0.9)
+    outs = _poisoned(L.allocate_outputs("distill_topk_forward", (x, teacher, weight)))
+    _launch("distill_topk_forward", (x, teacher, weight), outs)
+    w, rest = weight.double(), 1.0 - weight.double().exp().sum(-1)
+    outside = torch.logsumexp(logp.scatter(1, teacher, -math.inf), -1)
+    loss = (w.exp() * (w - logp.gather(1, teacher))).sum(-1) + rest * (rest.log() - outside)
+    assert float((outs[0] - loss).abs().max()) < 3 * e_sum + 24 * U * 60
+    (grad,) = L.allocate_outputs("distill_topk_backward", (x,))
+    _launch("distill_topk_backward", (x, teacher, weight, outs[1], g), (grad,))
+    want = (logp - outside[:, None]).exp() * (outside.exp() - rest)[:, None]
+    want.scatter_(1, teacher, logp.gather(1, teacher).exp() - w.exp())
+    want *= g[:, None].double()
+    size = (logp - outside[:, None]).exp() + logp.exp()
+    size.scatter_add_(1, teacher, w.exp())
+    tol = size * U * (64 + 32 * 40 + 1536) + want.abs() * (2.0 ** -8 if dtype == torch.bfloat16 else 0.0) + 1e-37
+    assert bool(((grad.double() - want).abs() <= tol).all())
+    assert N.device_status() == 0
+
+
+def test_first_launch_of_a_form_inside_a_capture(native_lib):
+    """The device's first call sets the library up; any other form of a kernel may then meet its first launch in a
+    capture."""
+    warm = torch.zeros(2, 64, device=DEV)
+    L.launch_token_logprobs_forward((warm, None), L.allocate_outputs("token_logprobs_forward", (warm, None)))
+    x, targets = _logits(3, 777, torch.bfloat16, 72)
+    index, value = _teacher(x, 5, 73)
+    logits, targets_d, index_d, value_d = (t.to(DEV) for t in (x, targets, index, value))
+    outs = L.allocate_outputs("token_logprobs_forward", (logits, targets_d), top_k=7)
+    kd = L.allocate_outputs("distill_topk_forward", (logits,))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        L.launch_token_logprobs_forward((logits, targets_d), outs, cluster_size=2)
+        L.launch_distill_topk_forward((logits, index_d, value_d), kd, cluster_size=2, tail=False)
+    graph.replay()
+    torch.cuda.synchronize()
+    _check_logprobs(x, targets, outs, 1.0, 7)
