@@ -7,8 +7,8 @@
 // (src/workloads/softmax_logits_backward.cu:410).
 //
 // Both directions are bound by HBM, the forward pass with the exponential unit at two thirds beside it: bf16 on one
-// B200, 4096 x 131072 with entropy 164-170 us = 6.0-6.2 TB/s (4 CTAs of 256 threads an SM; a chunk of four vectors a thread
-// with the next one in flight), with 20 alternatives 211 us; the gradient of 4096 x 65536 155 us = 6.7 TB/s. Eight rows of
+// B200, 4096 x 131072 with entropy 164-170 us = 6.0-6.2 TB/s (1024 threads an SM, 128 or 256 a row; a chunk of four vectors
+// a thread with the next one in flight), with 20 alternatives 211 us; the gradient of 4096 x 65536 155 us = 6.7 TB/s. Eight rows of
 // 131072 with 20 alternatives take 10 us: latency of a selection in each CTA and one over the cluster.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -94,9 +94,10 @@ __device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, con
 // ---------------------------------------------------------------------------
 // forward: one cluster per row, the row read once
 // ---------------------------------------------------------------------------
-template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const LogprobArgs a) {
-    __shared__ SoftmaxRecord warp_records[kThreads / 32];
+template <typename T, bool ENTROPY, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const LogprobArgs a) {
+    static_assert(!TOP || THREADS == kTopThreads, "the selection's CTA");
+    __shared__ SoftmaxRecord warp_records[THREADS / 32];
     __shared__ SoftmaxRecord records[kMaxClusterSize];   // rank 0: one per CTA
     __shared__ float row_max, row_log_sum;
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
     const int start = static_cast<int>(rank) * a.slice;
     const RowSpan<T> span(x, start, max(0, min(a.slice, a.cols - start)));
     uint4 ahead[kUnroll];
-    fetch_chunk<T, kThreads, kUnroll>(span, 0, ahead);
+    fetch_chunk<T, THREADS, kUnroll>(span, 0, ahead);
     const float edge = edge_element(span);
     cluster_arrive_release();   // "this CTA runs": its shared memory may be written from now on
     const float picked = rank == 0 && tid == 0 ? target_logit(a, x, target) : 0.0f;
@@ -126,9 +127,9 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
 
     const float k2 = a.inv_t * kLog2e;
     SoftmaxRecord rec = empty_record();
-    const int chunks = chunks_of<T, kThreads, kUnroll>(span);
+    const int chunks = chunks_of<T, THREADS, kUnroll>(span);
     TopCollector<T, kUnroll> collector(t, a.top_k, chunks);
-    stream_chunks<T, kThreads, kUnroll>(span, ahead, [&](const uint4 (&v)[kUnroll], int it) {
+    stream_chunks<T, THREADS, kUnroll>(span, ahead, [&](const uint4 (&v)[kUnroll], int it) {
         const float top = chunk_max<T>(v);
         if (TOP) collector.add(top, it);
         accumulate<T, kUnroll, ENTROPY>(v, top, k2, rec);
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Logpr
         accumulate<T, 1, ENTROPY>(v, edge, k2, rec);
     }
     const float thread_max = rec.m;
-    rec = cta_record<kThreads>(rec, warp_records, k2);   // its barrier also lies behind the buffer's set-up
+    rec = cta_record<THREADS>(rec, warp_records, k2);   // its barrier also lies behind the buffer's set-up
     if (TOP) {
         if (tid < span.edges) collector.add_edge(edge, span.start + span.edge_offset(tid));
         collector.finish(span, thread_max);
@@ -241,13 +242,16 @@ __global__ void __launch_bounds__(kThreads, 6) token_logprobs_bwd_kernel(const L
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+template <typename T, bool ENTROPY>
+const void* forward_kernel(bool top, int threads) {
+    if (top) return reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, true, kThreads>);
+    return threads == kThreads ? reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, false, kThreads>)
+                               : reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, false, kThreads / 2>);
+}
+
 template <typename T>
-const void* forward_kernel(bool entropy, bool top) {
-    if (entropy)
-        return top ? reinterpret_cast<const void*>(&token_logprobs_kernel<T, true, true>)
-                   : reinterpret_cast<const void*>(&token_logprobs_kernel<T, true, false>);
-    return top ? reinterpret_cast<const void*>(&token_logprobs_kernel<T, false, true>)
-               : reinterpret_cast<const void*>(&token_logprobs_kernel<T, false, false>);
+const void* forward_kernel(bool entropy, bool top, int threads) {
+    return entropy ? forward_kernel<T, true>(top, threads) : forward_kernel<T, false>(top, threads);
 }
 
 template <typename T>
@@ -296,14 +300,18 @@ int forward(const void* logits, int64_t ld, const int64_t* targets, float* logpr
     a.inv_t = 1.0f / temperature;
     a.status = ctx.status;
     const bool top = top_k > 0;
-    const void* func = dtype == CREDIT_BF16 ? forward_kernel<__nv_bfloat16>(entropy != nullptr, top)
-                                            : forward_kernel<float>(entropy != nullptr, top);
+    // Half as many threads a row let twice as many rows overlap, whose reductions and ends are then hidden, once the rows
+    // fill the eight CTAs an SM that fit: bf16 8192 x 16384 67 -> 53 us, 8192 x 2048 45 -> 25, 4096 x 131072 169 -> 168.
+    // With fewer rows the CTAs with more loads in flight win: 900 x 131072 44 us against 50, 300 x 131072 24 against 32.
+    const int threads = !top && cluster == 1 && rows >= 8 * ctx.sm_count ? kThreads / 2 : kThreads;
+    const void* func = dtype == CREDIT_BF16 ? forward_kernel<__nv_bfloat16>(entropy != nullptr, top, threads)
+                                            : forward_kernel<float>(entropy != nullptr, top, threads);
     rc = prepare_kernel(ctx, func);
     if (rc != CREDIT_OK) return rc;
     void* args[] = {&a};
     // the candidates, and in a cluster the lists that rank 0 gathers
     const size_t smem = top ? sizeof(TopBuffer) + (cluster > 1 ? sizeof(uint64_t) * cluster * top_k : 0) : 0;
-    return launch_kernel(func, rows * cluster, kThreads, cluster, static_cast<int>(smem), stream, args);
+    return launch_kernel(func, rows * cluster, threads, cluster, static_cast<int>(smem), stream, args);
 }
 
 int backward(const void* logits, int64_t ld, const int64_t* targets, const float* stats, const float* entropy,

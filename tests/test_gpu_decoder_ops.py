@@ -354,6 +354,28 @@ def test_many_rows_with_masks_and_special_values(native_lib, dtype):
     assert N.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,ld,shift", [(1184, 1, None, 0), (1300, 37, 40, 1), (1300, 4099, None, 5),
+                                                (1201, 8200, 8260, 1), (1500, 1031, None, 0)])
+@pytest.mark.parametrize("entropy", [True, False])
+def test_as_many_rows_as_fill_the_device(native_lib, dtype, rows, cols, ld, shift, entropy):
+    """Rows of every kind next to one another, without alternatives, at lengths below and above a CTA's chunk."""
+    x, targets = _logits(rows, cols, dtype, rows + cols)
+    x[1::9] = -math.inf
+    x[2::9, cols // 3 + 1:] = -math.inf
+    x[3::9] = torch.finfo(dtype).min
+    x[4::9, cols // 2] = NAN
+    x[5::9, cols - 1] = math.inf
+    x[6::9] = torch.arange(cols).to(dtype)
+    x[7::9] = 1.5
+    targets[8::9] = -1
+    x[8::18] = NAN
+    clean = x.clone()
+    clean[targets < 0] = 0.0
+    _check_logprobs(clean, targets, _run_logprobs(x, targets, 0, 0.8, 0, ld, shift, entropy), 0.8, 0)
+    assert N.device_status() == 0
+
+
 def test_token_logprobs_ignored_and_bad_targets(native_lib):
     x, targets = _logits(5, 700, torch.float32, 3)
     targets[1], targets[4] = -1, -100
