@@ -31,6 +31,8 @@ NAN = float("nan")
 def _within(got, want, tol, what=""):
     """|got - want| <= tol where want is finite; equal infinities and NaN elsewhere."""
     got, want = got.detach().cpu().double(), want.double()
+    # beyond fp32's largest value and half a step, its infinities
+    want = torch.where(want.abs() >= 2.0 ** 128 - 2.0 ** 103, want.sign() * math.inf, want)
     tol = torch.as_tensor(tol, dtype=torch.float64).expand_as(want)
     assert torch.equal(torch.isnan(got), torch.isnan(want)), what
     special = ~torch.isfinite(want)
@@ -376,6 +378,46 @@ def test_as_many_rows_as_fill_the_device(native_lib, dtype, rows, cols, ld, shif
     assert N.device_status() == 0
 
 
+def _far_rows(dtype, cols, seed):
+    """Rows far from zero: log2(e) times their maximum is large, near 2^24, or beyond fp32's resolution of 1."""
+    x, targets = _logits(10, cols, torch.float32, seed)
+    x[0] = -1e9                     # a finite mask that leaves nothing
+    x[1] = -1e10
+    x[2] = -1e20
+    x[3] += 1e10
+    x[4, cols // 2:] = -1e10
+    step = torch.arange(cols) % 24  # maxima on both sides of 2^24 / log2(e)
+    x[5] = 11629068.0 + step
+    x[6] = -11629090.0 + step
+    x[7] = 11629068.0 + 24.0 * torch.arange(cols) / cols
+    x[8] = 3e38
+    x[9] = 1e25 * torch.arange(cols)
+    return x.to(dtype), targets
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols,cluster,top_k", [(9001, 1, 0), (9001, 4, 0), (9001, 1, 12), (257, 0, 3)])
+def test_token_logprobs_rows_far_from_zero(native_lib, dtype, cols, cluster, top_k):
+    x, targets = _far_rows(dtype, cols, 90)
+    _check_logprobs(x, targets, _run_logprobs(x, targets, top_k, 1.0, cluster), 1.0, top_k)
+    assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1e-12, 1e-9, 1e-6, 1e6, 1e12, 1e22])
+def test_token_logprobs_extreme_temperatures(native_lib, dtype, temperature):
+    """Logits on the temperature's own scale, some masked, and (near greedy) on the ordinary one."""
+    x, targets = _logits(6, 5003, torch.float32, 91)
+    x[:4] *= temperature
+    x = x.to(dtype)
+    x[1::2, 7::3] = -math.inf
+    x[3, :] = torch.where(x[3] < 0, torch.finfo(dtype).min, x[3].double()).to(dtype)
+    for cluster in (1, 4):
+        _check_logprobs(x, targets, _run_logprobs(x, targets, 5, temperature, cluster), temperature, 5)
+    _check_logprob_gradient(x[:4], targets[:4], temperature, True)
+    assert N.device_status() == 0
+
+
 def test_token_logprobs_ignored_and_bad_targets(native_lib):
     x, targets = _logits(5, 700, torch.float32, 3)
     targets[1], targets[4] = -1, -100
@@ -571,6 +613,21 @@ def test_distill_many_rows(native_lib, tail):
     x[8::11, 5] = NAN
     x[9::11, cols - 1] = math.inf
     _check_distill(x, index, logprob, 1.0, tail)
+    assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [True, False])
+@pytest.mark.parametrize("cluster", [1, 4])
+def test_distill_rows_far_from_zero(native_lib, dtype, tail, cluster):
+    x, _ = _far_rows(dtype, 9001, 92)
+    index, logprob = _teacher(_logits(10, 9001, torch.float32, 93)[0], 8, 94)
+    _check_distill(x, index, logprob, 1.0, tail, cluster)
+    x, _ = _logits(4, 5003, torch.float32, 95)
+    x[1::2, 7::3] = -math.inf
+    index, logprob = _teacher(x, 8, 96)
+    for temperature in (1e-9, 1e12):
+        _check_distill((x * temperature).to(dtype), index, logprob, temperature, tail, cluster)
     assert N.device_status() == 0
 
 
