@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_bwd_kern
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int e = e0 + u * kStride;
-            if (W == 1 && sizeof(T) == 2 && u * kStride >= local) break;   // 374 -> 338 us at 16384 x 5003
+        if (W == 1 && sizeof(T) == 2 && u * kStride >= local) break;   // 374 -> 338 us at 16384 x 5003
 #pragma unroll
         for (int j = 0; j < W; ++j) c[u][j] = w[u][j] = col_c[u][j] = col_w[u][j] = 0.0f;
         if (e < local) {
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_bwd_kern
 #pragma unroll
     for (int u = 0; u < N; ++u) {
         const int e = e0 + u * kStride;
-            if (W == 1 && sizeof(T) == 2 && u * kStride >= local) break;
+        if (W == 1 && sizeof(T) == 2 && u * kStride >= local) break;
         if (e < local) {
             store_elems<float, W>(sums_out + e, col_c[u]);
             store_elems<float, W>(sums_out + a.ring.cols + e, col_w[u]);
