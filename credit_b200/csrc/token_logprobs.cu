@@ -7,8 +7,8 @@
 // (src/workloads/softmax_logits_backward.cu:410).
 //
 // Both directions are bound by HBM, the forward pass with the exponential unit at two thirds beside it: bf16 on one
-// B200, 4096 x 131072 with entropy 164-170 us = 6.0-6.2 TB/s (1024 threads an SM, 128 or 256 a row; a chunk of four vectors
-// a thread with the next one in flight), with 20 alternatives 211 us; the gradient of 4096 x 65536 155 us = 6.7 TB/s. Eight rows of
+// B200, 4096 x 131072 with entropy 161 us = 6.35 TB/s (1024 threads an SM, 128 or 256 a row; a chunk of four vectors
+// a thread with the next one in flight), with 20 alternatives 205 us; the gradient of 4096 x 65536 155 us = 6.7 TB/s. Eight rows of
 // 131072 with 20 alternatives take 10 us: latency of a selection in each CTA and one over the cluster.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -22,7 +22,7 @@
 namespace credit {
 namespace {
 
-constexpr int kThreads = kTopThreads;
+constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
 
 struct LogprobArgs {
@@ -80,7 +80,8 @@ __device__ __forceinline__ float write_row(const LogprobArgs& a, int64_t row, co
 }
 
 // The sorted alternatives in t.keys, by the threads of one CTA.
-__device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, const TopBuffer& t, float row_max,
+template <int THREADS>
+__device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, const TopBuffer<THREADS>& t, float row_max,
                                           float row_log_sum) {
     const int tid = threadIdx.x;
     if (tid >= a.top_k) return;
@@ -96,12 +97,11 @@ __device__ __forceinline__ void write_top(const LogprobArgs& a, int64_t row, con
 // ---------------------------------------------------------------------------
 template <typename T, bool ENTROPY, bool TOP, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const LogprobArgs a) {
-    static_assert(!TOP || THREADS == kTopThreads, "the selection's CTA");
     __shared__ SoftmaxRecord warp_records[THREADS / 32];
     __shared__ SoftmaxRecord records[kMaxClusterSize];   // rank 0: one per CTA
     __shared__ float row_max, row_log_sum;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    TopBuffer& t = *reinterpret_cast<TopBuffer*>(dynamic);
+    TopBuffer<THREADS>& t = *reinterpret_cast<TopBuffer<THREADS>*>(dynamic);
 
     const uint32_t rank = cluster_cta_rank(), nranks = cluster_cta_count();
     const int64_t row = blockIdx.x / nranks;
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     const float k2 = a.inv_t * kLog2e;
     SoftmaxRecord rec = empty_record();
     const int chunks = chunks_of<T, THREADS, kUnroll>(span);
-    TopCollector<T, kUnroll> collector(t, a.top_k, chunks);
+    TopCollector<T, THREADS, kUnroll> collector(t, a.top_k, chunks);
     stream_chunks<T, THREADS, kUnroll>(span, ahead, [&](const uint4 (&v)[kUnroll], int it) {
         const float top = chunk_max<T>(v);
         if (TOP) collector.add(top, it);
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
             st_cluster_u64(map_to_rank(smem_u32(&gathered[rank * a.top_k + tid]), 0), tid < t.fill ? t.keys[tid] : 0);
         cluster_sync_all();
         if (rank != 0) return;
-        if (TOP) merge_lists(t, gathered, static_cast<int>(nranks), a.top_k);
+        if constexpr (TOP && THREADS == kThreads) merge_lists(t, gathered, static_cast<int>(nranks), a.top_k);
         if (tid < 32) {
             if (tid == 0) records[0] = rec;
             __syncwarp();
@@ -244,9 +244,11 @@ __global__ void __launch_bounds__(kThreads, 6) token_logprobs_bwd_kernel(const L
 // ---------------------------------------------------------------------------
 template <typename T, bool ENTROPY>
 const void* forward_kernel(bool top, int threads) {
-    if (top) return reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, true, kThreads>);
-    return threads == kThreads ? reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, false, kThreads>)
-                               : reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, false, kThreads / 2>);
+    if (threads == kThreads)
+        return top ? reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, true, kThreads>)
+                   : reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, false, kThreads>);
+    return top ? reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, true, kThreads / 2>)
+               : reinterpret_cast<const void*>(&token_logprobs_kernel<T, ENTROPY, false, kThreads / 2>);
 }
 
 template <typename T>
@@ -300,17 +302,20 @@ int forward(const void* logits, int64_t ld, const int64_t* targets, float* logpr
     a.inv_t = 1.0f / temperature;
     a.status = ctx.status;
     const bool top = top_k > 0;
-    // Half as many threads a row let twice as many rows overlap, whose reductions and ends are then hidden, once the rows
-    // fill the eight CTAs an SM that fit: bf16 8192 x 16384 67 -> 53 us, 8192 x 2048 45 -> 25, 4096 x 131072 169 -> 168.
-    // With fewer rows the CTAs with more loads in flight win: 900 x 131072 44 us against 50, 300 x 131072 24 against 32.
-    const int threads = !top && cluster == 1 && rows >= 8 * ctx.sm_count ? kThreads / 2 : kThreads;
+    // Half as many threads a row let twice as many rows overlap, whose reductions, selections and ends are then hidden,
+    // once the rows fill the eight CTAs an SM that fit: bf16 8192 x 16384 67 -> 51 us, 8192 x 2048 45 -> 24, 4096 x 131072
+    // 169 -> 161; with 20 alternatives 8192 x 16384 135 -> 93, 8192 x 32768 169 -> 129, 4096 x 131072 203 / 206 (1184
+    // such rows 68 / 73). With fewer rows the CTAs with more loads in flight win (900 x 131072 43 us against 50, 300 x 131072 23 against 32), and
+    // so do those with more maxima to bound many alternatives by (64 of 4096 x 131072: 230 against 256).
+    const int threads = cluster == 1 && rows >= 8 * ctx.sm_count && top_k <= 32 ? kThreads / 2 : kThreads;
     const void* func = dtype == CREDIT_BF16 ? forward_kernel<__nv_bfloat16>(entropy != nullptr, top, threads)
                                             : forward_kernel<float>(entropy != nullptr, top, threads);
     rc = prepare_kernel(ctx, func);
     if (rc != CREDIT_OK) return rc;
     void* args[] = {&a};
     // the candidates, and in a cluster the lists that rank 0 gathers
-    const size_t smem = top ? sizeof(TopBuffer) + (cluster > 1 ? sizeof(uint64_t) * cluster * top_k : 0) : 0;
+    const size_t buffer = threads == kThreads ? sizeof(TopBuffer<kThreads>) : sizeof(TopBuffer<kThreads / 2>);
+    const size_t smem = top ? buffer + (cluster > 1 ? sizeof(uint64_t) * cluster * top_k : 0) : 0;
     return launch_kernel(func, rows * cluster, threads, cluster, static_cast<int>(smem), stream, args);
 }
 

@@ -1,8 +1,8 @@
 // The k largest of a row slice that is read once. While it streams by, every thread stores the maximum of each
 // group of its elements (32 bf16 or 16 fp32 a chunk; as many chunks a group as make at most 16 groups): one store
-// and nothing else. At the end every warp takes its ceil(k / 8)-th largest thread maximum; the smallest of the
-// eight has k elements that reach it, about 50 (k = 20) to 250 (k = 128) groups do, and those are read again: their
-// elements that reach it compete by rank.
+// and nothing else. At the end each of W warps takes its ceil(k / W)-th largest thread maximum; the smallest of the
+// W has k elements that reach it, about 50 (k = 20) to 250 (k = 128) groups do in 8 warps, and those are read again:
+// their elements that reach it compete by rank.
 //
 // Order. An element is the 64-bit key (monotone image of its value, complement of its column): larger
 // keys first is "value descending, column ascending", all keys of a row differ, so the chosen set
@@ -22,8 +22,6 @@
 namespace credit {
 
 constexpr int kMaxTop = 128;
-constexpr int kTopThreads = 256;
-constexpr int kTopCapacity = 2048;
 constexpr int kTopGroups = 16;   // a thread's
 constexpr uint64_t kLowestKey = 0x0080000000000000ull;   // the image of -FLT_MAX, any column
 
@@ -34,27 +32,31 @@ __device__ __forceinline__ uint64_t element_key(float x, int column) {
 __device__ __forceinline__ float key_value(uint64_t key) { return image_value(static_cast<uint32_t>(key >> 32)); }
 __device__ __forceinline__ int key_column(uint64_t key) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key)); }
 
+template <int THREADS>
 struct TopBuffer {
-    unsigned long long keys[kTopCapacity];
+    static constexpr int kPlaces = 8 * THREADS;
+    unsigned long long keys[kPlaces];
     unsigned int hist[256];
     unsigned long long lowest;   // smallest kept key
-    float group[kTopGroups][kTopThreads];   // maxima
-    unsigned int floor[kTopThreads / 32];   // image of each warp's share of the threshold
+    float group[kTopGroups][THREADS];   // maxima
+    unsigned int floor[THREADS / 32];   // image of each warp's share of the threshold
     unsigned int differ[2];      // bits in which the keys differ (high, low word); zero between calls
-    int noted[kTopCapacity];     // groups that reach the threshold
+    int noted[kPlaces];          // groups that reach the threshold
     int notes;                   // (may exceed the places, like count)
     int count;                   // candidates appended
     int fill, digit, above, here;
 };
 
 // By one thread, before the first barrier.
-__device__ __forceinline__ void init_top_buffer(TopBuffer& t) {
+template <int THREADS>
+__device__ __forceinline__ void init_top_buffer(TopBuffer<THREADS>& t) {
     t.count = t.notes = 0;
     t.differ[0] = t.differ[1] = 0;
 }
 
 // Warp 0: the digit in which the need-th largest lies, how many lie above it and in it.
-__device__ __forceinline__ void find_digit(TopBuffer& t, int need) {
+template <int THREADS>
+__device__ __forceinline__ void find_digit(TopBuffer<THREADS>& t, int need) {
     const int lane = threadIdx.x & 31;
     int part[8], sum = 0;
 #pragma unroll
@@ -82,18 +84,19 @@ __device__ __forceinline__ void find_digit(TopBuffer& t, int need) {
     }
 }
 
-// Keeps the k largest of keys[0, n), n <= kTopCapacity (fewer when fewer are non-zero: zeros are
+// Keeps the k largest of keys[0, n), n <= kPlaces (fewer when fewer are non-zero: zeros are
 // empty places), and returns the smallest of them (0 when there are fewer than k). All threads call
 // it behind a barrier; it ends with one, the number kept in t.fill.
-__device__ __forceinline__ uint64_t keep_largest(TopBuffer& t, int n, int k) {
-    constexpr int kPer = kTopCapacity / kTopThreads;
+template <int THREADS>
+__device__ __forceinline__ uint64_t keep_largest(TopBuffer<THREADS>& t, int n, int k) {
+    constexpr int kPer = TopBuffer<THREADS>::kPlaces / THREADS;
     const int tid = threadIdx.x;
     uint64_t mine[kPer];
     const uint64_t some = t.keys[0];
     uint64_t diff = 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        const int i = tid + j * kTopThreads;
+        const int i = tid + j * THREADS;
         mine[j] = i < n ? t.keys[i] : some;
         diff |= mine[j] ^ some;
         if (i >= n) mine[j] = 0;
@@ -115,11 +118,11 @@ __device__ __forceinline__ uint64_t keep_largest(TopBuffer& t, int n, int k) {
         while (bits > 0) {
             const int shift = bits > 8 ? bits - 8 : 0;
             const uint32_t digits = (1u << (bits - shift)) - 1u;
-            t.hist[tid] = 0;
+            for (int i = tid; i < 256; i += THREADS) t.hist[i] = 0;
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < kPer; ++j)
-                if (tid + j * kTopThreads < n && ((mine[j] ^ threshold) & mask) == 0)
+                if (tid + j * THREADS < n && ((mine[j] ^ threshold) & mask) == 0)
                     atomicAdd(&t.hist[static_cast<uint32_t>(mine[j] >> shift) & digits], 1u);
             __syncthreads();
             if (tid < 32) find_digit(t, need);
@@ -152,15 +155,16 @@ __device__ __forceinline__ uint64_t keep_largest(TopBuffer& t, int n, int k) {
 
 // The same, sorted descending: with one key a thread at most, the larger ones are counted for each, which is
 // its place; more go through the digits first. Returns the k-th (0 when there are fewer).
-__device__ __noinline__ uint64_t rank_largest(TopBuffer& t, int n, int k) {
+template <int THREADS>
+__device__ __noinline__ uint64_t rank_largest(TopBuffer<THREADS>& t, int n, int k) {
     const int tid = threadIdx.x;
-    if (n > kTopThreads) {
+    if (n > THREADS) {
         keep_largest(t, n, k);
         n = t.fill;
         __syncthreads();
     }
     // few keys: 4 or 2 neighbouring threads share one and count a part of the others each
-    const int shift = n <= kTopThreads / 4 ? 2 : (n <= kTopThreads / 2 ? 1 : 0), share = 1 << shift;
+    const int shift = n <= THREADS / 4 ? 2 : (n <= THREADS / 2 ? 1 : 0), share = 1 << shift;
     const int at = tid >> shift, part = tid & (share - 1);
     const uint64_t mine = at < n ? t.keys[at] : 0;
     int place = 0;
@@ -184,16 +188,16 @@ __device__ __noinline__ uint64_t rank_largest(TopBuffer& t, int n, int k) {
 
 // The slow path: the same selection straight from the slice in global memory. Leaves at most k keys
 // in keys[0, fill) and ends with a barrier.
-template <typename T>
-__device__ __noinline__ void select_from_slice(const T* first, int start, int local, int k, TopBuffer& t) {
+template <typename T, int THREADS>
+__device__ __noinline__ void select_from_slice(const T* first, int start, int local, int k, TopBuffer<THREADS>& t) {
     const int tid = threadIdx.x;
     uint64_t threshold = 0, mask = 0;
     int need = k;
     for (int shift = 56; shift >= 0; shift -= 8) {
-        t.hist[tid] = 0;
+        for (int i = tid; i < 256; i += THREADS) t.hist[i] = 0;
         if (tid == 0) t.digit = -1;
         __syncthreads();
-        for (int base = 0; base < local; base += kTopThreads) {
+        for (int base = 0; base < local; base += THREADS) {
             int digit = -1;
             if (base + tid < local) {
                 const uint64_t key = element_key(Vec<T>::load(first + base + tid), start + base + tid);
@@ -222,26 +226,26 @@ __device__ __noinline__ void select_from_slice(const T* first, int start, int lo
     if (threshold < kLowestKey) threshold = kLowestKey;
     if (tid == 0) t.fill = 0;
     __syncthreads();
-    for (int c = tid; c < local; c += kTopThreads) {
+    for (int c = tid; c < local; c += THREADS) {
         const uint64_t key = element_key(Vec<T>::load(first + c), start + c);
         if (key >= threshold) {
             const int at = atomicAdd(&t.fill, 1);
-            if (at < kTopCapacity) t.keys[at] = key;
+            if (at < TopBuffer<THREADS>::kPlaces) t.keys[at] = key;
         }
     }
     __syncthreads();
 }
 
 // One CTA's groups while its slice streams by, in chunks of U vectors a thread.
-template <typename T, int U>
+template <typename T, int THREADS, int U>
 struct TopCollector {
-    static constexpr int E = Vec<T>::kElems;
-    TopBuffer& t;
+    static constexpr int E = Vec<T>::kElems, kWarps = THREADS / 32, kPlaces = TopBuffer<THREADS>::kPlaces;
+    TopBuffer<THREADS>& t;
     const int k;
     int chunks, per_group;
     float running;
 
-    __device__ __forceinline__ TopCollector(TopBuffer& t_, int k_, int chunks_)
+    __device__ __forceinline__ TopCollector(TopBuffer<THREADS>& t_, int k_, int chunks_)
         : t(t_), k(k_), chunks(chunks_), per_group((chunks_ + kTopGroups - 1) / kTopGroups), running(-INFINITY) {}
 
     // The thread's maximum of chunk `it`.
@@ -256,7 +260,7 @@ struct TopCollector {
 
     __device__ __forceinline__ void offer(float x, int column) {
         const int at = atomicAdd(&t.count, 1);
-        if (at < kTopCapacity) t.keys[at] = element_key(x, column);
+        if (at < kPlaces) t.keys[at] = element_key(x, column);
     }
 
     // An element outside the vectors competes in any case.
@@ -272,13 +276,13 @@ struct TopCollector {
         uint32_t m = 0;
         bool taken = false;
 #pragma unroll 1
-        for (int i = 0; i < (k + 7) / 8; ++i) {
+        for (int i = 0; i < (k + kWarps - 1) / kWarps; ++i) {
             m = __reduce_max_sync(0xffffffffu, taken ? 0u : mine);
             taken |= lane == __ffs(__ballot_sync(0xffffffffu, !taken && mine == m)) - 1;
         }
         if (lane == 0) t.floor[tid >> 5] = m;
         __syncthreads();
-        const uint32_t least = max(__reduce_min_sync(0xffffffffu, t.floor[lane & (kTopThreads / 32 - 1)]),
+        const uint32_t least = max(__reduce_min_sync(0xffffffffu, t.floor[lane & (kWarps - 1)]),
                                    static_cast<uint32_t>(kLowestKey >> 32));
         const float floor = image_value(least);   // NaN: only NaN reaches it
         const bool nan = floor != floor;
@@ -292,16 +296,16 @@ struct TopCollector {
         if (reach != 0) {
             int at = atomicAdd(&t.notes, __popc(reach));
             for (; reach != 0; reach &= reach - 1, ++at)
-                if (at < kTopCapacity) t.noted[at] = (__ffs(reach) - 1) * kTopThreads + tid;
+                if (at < kPlaces) t.noted[at] = (__ffs(reach) - 1) * THREADS + tid;
         }
         __syncthreads();
         const int notes = t.notes, vectors = U * per_group;
-        bool overflow = notes > kTopCapacity;
+        bool overflow = notes > kPlaces;
         if (!overflow) {
 #pragma unroll 1
-            for (int i = tid; i < notes * vectors; i += kTopThreads) {
+            for (int i = tid; i < notes * vectors; i += THREADS) {
                 const int which = per_group == 1 ? i / U : i / vectors, place = i - which * vectors, note = t.noted[which];
-                const int v = ((note / kTopThreads * per_group) * U + place) * kTopThreads + note % kTopThreads;
+                const int v = ((note / THREADS * per_group) * U + place) * THREADS + note % THREADS;
                 if (v >= span.nvec) continue;
                 float x[E];
                 Vec<T>::unpack(span.vectors()[v], x);
@@ -315,14 +319,14 @@ struct TopCollector {
 #pragma unroll
                 for (int j = 0; j < E; ++j)
                     if (hits >> j & 1u) {
-                        if (at < kTopCapacity) t.keys[at] = element_key(x[j], column + j);
+                        if (at < kPlaces) t.keys[at] = element_key(x[j], column + j);
                         ++at;
                     }
             }
         }
         __syncthreads();
         int n = t.count;
-        if (overflow || n > kTopCapacity) {
+        if (overflow || n > kPlaces) {
             __syncthreads();
             select_from_slice(span.first, span.start, span.local, k, t);
             n = t.fill;
@@ -343,13 +347,15 @@ __device__ __forceinline__ uint64_t warp_min_key(uint64_t key) {
 // Rank 0: the k largest of `lists` sorted lists of k keys (zeros at their ends) into t.keys[0, fill), sorted. Of
 // every list the first ceil(k / lists) entries are k together, so nothing below the smallest of those can
 // be among the k largest. All threads, behind a barrier.
-__device__ __forceinline__ void merge_lists(TopBuffer& t, const unsigned long long* gathered, int lists, int k) {
+template <int THREADS>
+__device__ __forceinline__ void merge_lists(TopBuffer<THREADS>& t, const unsigned long long* gathered, int lists, int k) {
+    static_assert(TopBuffer<THREADS>::kPlaces >= kMaxClusterSize * kMaxTop, "every gathered key may be a candidate");
     const int share = (k + lists - 1) / lists - 1;
     const int lane = threadIdx.x & 31;
     const uint64_t floor = warp_min_key(lane < lists ? gathered[lane * k + share] : ~0ull);
     if (threadIdx.x == 0) t.count = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < lists * k; i += kTopThreads) {
+    for (int i = threadIdx.x; i < lists * k; i += THREADS) {
         const uint64_t key = gathered[i];
         if (key != 0 && key >= floor) t.keys[atomicAdd(&t.count, 1)] = key;   // at most 16 * 128 of them
     }
@@ -357,6 +363,5 @@ __device__ __forceinline__ void merge_lists(TopBuffer& t, const unsigned long lo
     const int n = t.count;
     rank_largest(t, n, k);
 }
-static_assert(kTopCapacity >= kMaxClusterSize * kMaxTop, "every gathered key may be a candidate");
 
 }  // namespace credit

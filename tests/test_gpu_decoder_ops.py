@@ -362,6 +362,17 @@ def test_many_rows_with_masks_and_special_values(native_lib, dtype):
 @pytest.mark.parametrize("entropy", [True, False])
 def test_as_many_rows_as_fill_the_device(native_lib, dtype, rows, cols, ld, shift, entropy):
     """Rows of every kind next to one another, without alternatives, at lengths below and above a CTA's chunk."""
+    _check_mixed_rows(dtype, rows, cols, ld, shift, entropy, 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,ld,shift,top_k", [(1184, 1, None, 0, 3), (1300, 37, 40, 1, 32), (1300, 4099, None, 5, 20),
+                                                      (1201, 8200, 8260, 1, 31), (1190, 9001, None, 0, 33), (1500, 1031, None, 0, 1)])
+def test_alternatives_of_as_many_rows_as_fill_the_device(native_lib, dtype, rows, cols, ld, shift, top_k):
+    _check_mixed_rows(dtype, rows, cols, ld, shift, True, top_k)
+
+
+def _check_mixed_rows(dtype, rows, cols, ld, shift, entropy, top_k):
     x, targets = _logits(rows, cols, dtype, rows + cols)
     x[1::9] = -math.inf
     x[2::9, cols // 3 + 1:] = -math.inf
@@ -374,7 +385,7 @@ def test_as_many_rows_as_fill_the_device(native_lib, dtype, rows, cols, ld, shif
     x[8::18] = NAN
     clean = x.clone()
     clean[targets < 0] = 0.0
-    _check_logprobs(clean, targets, _run_logprobs(x, targets, 0, 0.8, 0, ld, shift, entropy), 0.8, 0)
+    _check_logprobs(clean, targets, _run_logprobs(x, targets, top_k, 0.8, 0, ld, shift, entropy), 0.8, top_k)
     assert N.device_status() == 0
 
 
