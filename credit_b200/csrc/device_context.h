@@ -8,6 +8,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/credit_b200.h"
 #include "error_state.h"
 
@@ -37,6 +39,15 @@ int check_matrix_shape(int64_t rows, int64_t cols, int dtype);
 int check_cluster_only(const credit_launch_opts* opts, int* cluster);
 
 inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// All of them (a NULL is).
+inline bool aligned_to(std::initializer_list<const void*> pointers, size_t bytes) {
+    for (const void* p : pointers)
+        if (!aligned_to(p, bytes)) return false;
+    return true;
+}
+
+inline int element_bytes(int dtype) { return dtype == CREDIT_BF16 ? 2 : 4; }
 
 // Nothing crosses the C boundary as an exception (the caches above allocate).
 template <typename F>

@@ -423,6 +423,8 @@ int check_list(const int64_t* index, const float* teacher, int top_k, int64_t ro
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "top_k must be in [1, %d] (got %d)", kMaxList, top_k);
     if (rows != 0 && (index == nullptr || teacher == nullptr))
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "teacher_index and teacher_logprob must not be NULL");
+    if (!aligned_to(index, sizeof(int64_t)) || !aligned_to(teacher, sizeof(float)))
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "teacher_index and teacher_logprob must be aligned to their elements");
     return CREDIT_OK;
 }
 
@@ -437,6 +439,8 @@ int forward(const void* logits, int64_t ld, const int64_t* index, const float* t
     if (rows == 0) return CREDIT_OK;
     if (loss == nullptr || stats == nullptr)
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "loss and stats must not be NULL");
+    if (!aligned_to({loss, stats}, sizeof(float)))
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "loss and stats must be aligned to their elements");
     DeviceContext ctx;
     rc = current_device_context(&ctx);
     if (rc != CREDIT_OK) return rc;
@@ -492,6 +496,8 @@ int backward(const void* logits, int64_t ld, const int64_t* index, const float* 
     if (rows == 0) return CREDIT_OK;
     if (stats == nullptr || dloss == nullptr)
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "stats and dloss must not be NULL");
+    if (!aligned_to({stats, dloss}, sizeof(float)))
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "stats and dloss must be aligned to their elements");
     DeviceContext ctx;
     rc = current_device_context(&ctx);
     if (rc != CREDIT_OK) return rc;

@@ -659,7 +659,7 @@ int round_to(int64_t v, int m) { return static_cast<int>((v + m - 1) / m * m); }
 // bytes for each of 512 threads), so that three stages of four inputs fit an SM; the automatic cluster is the
 // smallest that holds the row.
 int plan_shape(int64_t cols, int dtype, bool vector, int asked, Plan* p, const Form** form) {
-    const int size = dtype == CREDIT_BF16 ? 2 : 4, each = 32 / size;
+    const int size = element_bytes(dtype), each = 32 / size;
     const int64_t most = 512 * each;
     int cluster = asked;
     if (cluster == 0)
@@ -704,19 +704,20 @@ int plan_launch(int64_t rows, const void* func, int inputs, Plan* p) {
     return CREDIT_OK;
 }
 
-bool all_aligned(std::initializer_list<const void*> pointers) {
-    for (const void* p : pointers)
-        if (!aligned_to(p, 16)) return false;
-    return true;
-}
-
 bool any_null(std::initializer_list<const void*> pointers) {
     for (const void* p : pointers)
         if (p == nullptr) return true;
     return false;
 }
 
-bool rows_of_vectors(int64_t cols, int dtype) { return cols * (dtype == CREDIT_BF16 ? 2 : 4) % 16 == 0; }
+bool rows_of_vectors(int64_t cols, int dtype) { return cols * element_bytes(dtype) % 16 == 0; }
+
+// The bulk copies round a matrix's address down to 16 bytes by whole elements.
+int check_alignment(std::initializer_list<const void*> matrices, std::initializer_list<const void*> vectors, int dtype) {
+    if (!aligned_to(matrices, element_bytes(dtype)) || !aligned_to(vectors, sizeof(float)))
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "matrices and fp32 vectors must be aligned to their elements");
+    return CREDIT_OK;
+}
 
 int forward(const void* block, const void* residual, const float* post_weight, const float* gate, const float* pre_weight,
             void* residual_out, void* y, float* post_rstd, float* pre_rstd, int64_t rows, int64_t cols, float alpha,
@@ -728,7 +729,7 @@ int forward(const void* block, const void* residual, const float* post_weight, c
     if (!std::isfinite(alpha) || !(eps > 0.0f) || !std::isfinite(eps))
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "residual_scale must be finite, eps positive and finite");
     const bool vector = rows_of_vectors(cols, dtype) &&
-                        all_aligned({block, residual, post_weight, gate, pre_weight, residual_out, y});
+                        aligned_to({block, residual, post_weight, gate, pre_weight, residual_out, y}, 16);
     const Form* form = nullptr;
     Plan p;
     rc = plan_shape(cols, dtype, vector, asked, &p, &form);
@@ -738,6 +739,8 @@ int forward(const void* block, const void* residual, const float* post_weight, c
     if ((post_weight == nullptr) != (post_rstd == nullptr))
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "post_weight and post_rstd go together");
     if (y == residual_out) return report_error(CREDIT_ERR_INVALID_ARGUMENT, "y and residual_out must differ");
+    rc = check_alignment({block, residual, residual_out, y}, {post_weight, gate, pre_weight, post_rstd, pre_rstd}, dtype);
+    if (rc != CREDIT_OK) return rc;
     rc = plan_launch(rows, form->forward[post_weight != nullptr], 2, &p);
     if (rc != CREDIT_OK) return rc;
     NormFwdArgs a;
@@ -792,8 +795,11 @@ int backward(const void* dy, const void* dresidual_out, const void* block, const
     if ((post_weight == nullptr) != (post_rstd == nullptr))
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "post_weight and post_rstd go together");
     if (dblock == dresidual) return report_error(CREDIT_ERR_INVALID_ARGUMENT, "dblock and dresidual must differ");
-    const bool vector = rows_of_vectors(cols, dtype) && all_aligned({dy, dresidual_out, block, residual_out, post_weight,
-                                                                     gate, pre_weight, dblock, dresidual});
+    rc = check_alignment({dy, dresidual_out, block, residual_out, dblock, dresidual},
+                         {post_weight, gate, pre_weight, post_rstd, pre_rstd, dpost_weight, dgate, dpre_weight}, dtype);
+    if (rc != CREDIT_OK) return rc;
+    const bool vector = rows_of_vectors(cols, dtype) && aligned_to({dy, dresidual_out, block, residual_out, post_weight, gate,
+                                                                    pre_weight, dblock, dresidual}, 16);
     Plan p;
     rc = plan_backward(rows, cols, dtype, vector, post_weight != nullptr, asked, &p);
     if (rc != CREDIT_OK) return rc;

@@ -282,6 +282,8 @@ int forward(const void* logits, int64_t ld, const int64_t* targets, float* logpr
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "nothing is asked for: targets, entropy and top_k are all absent");
     if (top_k > 0 && (top_logprob == nullptr || top_index == nullptr))
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "top_k = %d needs top_logprob and top_index", top_k);
+    if (!aligned_to({targets, top_index}, sizeof(int64_t)) || !aligned_to({logprob, stats, entropy, top_logprob}, sizeof(float)))
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "every vector must be aligned to its elements");
     DeviceContext ctx;
     rc = current_device_context(&ctx);
     if (rc != CREDIT_OK) return rc;
@@ -334,6 +336,8 @@ int backward(const void* logits, int64_t ld, const int64_t* targets, const float
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "targets, stats and dlogprob must not be NULL");
     if (dentropy != nullptr && entropy == nullptr)
         return report_error(CREDIT_ERR_INVALID_ARGUMENT, "dentropy needs the entropy of the forward pass");
+    if (!aligned_to(targets, sizeof(int64_t)) || !aligned_to({stats, entropy, dlogprob, dentropy}, sizeof(float)))
+        return report_error(CREDIT_ERR_INVALID_ARGUMENT, "every vector must be aligned to its elements");
     DeviceContext ctx;
     rc = current_device_context(&ctx);
     if (rc != CREDIT_OK) return rc;

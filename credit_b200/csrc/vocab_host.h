@@ -10,8 +10,6 @@ namespace credit {
 
 constexpr int64_t kMaxLogitCols = 1 << 22;
 
-inline int element_bytes(int dtype) { return dtype == CREDIT_BF16 ? 2 : 4; }
-
 inline int check_logits(const void* logits, int64_t ld, int64_t rows, int64_t cols, float temperature, int dtype) {
     int rc = check_matrix_shape(rows, cols, dtype);
     if (rc != CREDIT_OK) return rc;

@@ -291,6 +291,9 @@ int credit_layernorm_backward_stats_static(const void* x, const void* dy, const 
 
 /* The end of a decoder --------------------------------------------------- */
 
+/* In this section an address that is not aligned to its elements (2 bytes for bf16, 4 for
+ * fp32, 8 for int64) gives CREDIT_ERR_INVALID_ARGUMENT; rows may start anywhere else. */
+
 /* The norms after and before a block, fused with the block's gate and the scaled
  * residual, for fp32 or bf16 [rows, cols] matrices and fp32 [cols] parameters:
  *   n = block * rsqrt(mean(block^2) + eps)            (block itself without post_weight)
