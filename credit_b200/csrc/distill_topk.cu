@@ -9,6 +9,7 @@
 // The sum outside the list is accumulated as such (listed columns are marked in a bitmap and skipped),
 // never as "all minus listed", so a student that has almost all of its mass in the list keeps q_r and
 // its gradient to full precision; w_r is taken in 64 bits for the same reason.
+// A renormalised list may lie anywhere (raw logits): its weights are taken from differences to its largest value.
 // No reference kernel exists for this; the row pass is that of token_logprobs.cu and bound as it is: bf16 on one B200,
 // 2048 x 131072 with a list of 64 97 us = 5.5 TB/s (fp32 159 us = 6.8 TB/s), the gradient 173 us = 6.2 TB/s.
 #include <cuda_bf16.h>
@@ -62,8 +63,9 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 struct TeacherList {
     int column[kMaxList];      // -1 = unused
     float value[kMaxList];
-    double mass;               // tail: sum of exp(value); no tail: of exp(value - log_norm) (1, or 0 for none)
-    float log_norm;            // no tail: log sum exp(value)
+    float top;                 // largest value
+    float base;
+    double sum;                // of exp(value - base): 0 for a list without mass
     int bad;                   // some column lies outside the row
     int any;                   // some place is used
 };
@@ -95,7 +97,7 @@ __device__ __forceinline__ void load_list(const DistillArgs& a, int64_t row, Tea
         top = max_nan(top, v[i]);
     }
     top = warp_max_nan(top);
-    const float base = TAIL || top == -CUDART_INF_F ? 0.0f : top;
+    const float base = top == -CUDART_INF_F || (TAIL && fabsf(top) < 600.0f) ? 0.0f : top;   // 64 bits hold exp(+-600)
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) sum += exp(static_cast<double>(v[i]) - base);
@@ -103,8 +105,9 @@ __device__ __forceinline__ void load_list(const DistillArgs& a, int64_t row, Tea
     bad = __any_sync(0xffffffffu, bad);
     any = __any_sync(0xffffffffu, any);
     if (lane == 0) {
-        l.log_norm = TAIL || sum == 0.0 ? 0.0f : static_cast<float>(base + log(sum));
-        l.mass = TAIL ? sum : (sum == 0.0 ? 0.0 : 1.0);
+        l.top = top;
+        l.base = base;
+        l.sum = sum;
         l.bad = bad;
         l.any = any;
     }
@@ -218,28 +221,32 @@ __device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, co
         mine.s = warp_sum(mine.s);
         all = merge_records(rec, mine, k2);
     }
-    const bool broken = is_broken(all.m) || list.bad;
+    const bool broken = is_broken(all.m) || list.bad || isnan(list.sum);
     const bool empty = all.m == -CUDART_INF_F, no_tail = rec.m == -CUDART_INF_F;
     const float log_sum = empty ? 0.0f : log_sum_of(all, k2);
     const float tail_log_sum = no_tail ? 0.0f : log_sum_of(rec, k2);
     // the teacher: always a distribution. Without anything left outside the student's list, or with a
-    // list of more than 1, it is renormalised over the list.
-    float log_norm = list.log_norm, rest = 0.0f;
+    // list of more than 1, it is renormalised over the list, by differences to the list's largest value: a
+    // normaliser far from zero has too few bits for exp(value - normaliser).
+    float top = 0.0f, shift = 0.0f, log_norm = 0.0f, rest = 0.0f;
     bool no_teacher = false;
-    if (TAIL) {
-        const double left = 1.0 - list.mass;
-        if (no_tail || left < 0.0) {
-            no_teacher = list.mass == 0.0;   // all of it outside the list, and nothing is there
-            log_norm = no_teacher ? 0.0f : static_cast<float>(log(list.mass));
-        } else {
-            rest = static_cast<float>(left);
+    const double left = TAIL ? 1.0 - (list.base == 0.0f ? list.sum : list.sum * exp(static_cast<double>(list.base))) : 0.0;
+    if (!TAIL || no_tail || left < 0.0) {
+        no_teacher = list.sum == 0.0;   // all of it outside the list, and nothing is there
+        if (!no_teacher) {
+            const double log_mass = list.base + log(list.sum);
+            top = list.top;
+            shift = static_cast<float>(log_mass - top);
+            log_norm = static_cast<float>(log_mass);
         }
+    } else {
+        rest = static_cast<float>(left);
     }
     double loss = 0.0;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
         const int k = lane + 32 * i;
-        const float logw = list.value[k] - log_norm;
+        const float logw = (list.value[k] - top) - shift;
         const float w = expf(logw);
         if (list.column[k] >= 0 && w != 0.0f) {
             const float logq = empty ? -CUDART_INF_F : (student[k] - all.m) * a.inv_t - log_sum;
@@ -290,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 8) distill_topk_kernel(const Distill
     if (TAIL)
         for (int i = tid; i < a.map_words / 4; i += kThreads) reinterpret_cast<uint4*>(map)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    if (!list.bad && (TAIL ? !list.any : list.mass == 0.0)) {
+    if (!list.bad && (TAIL ? !list.any : list.sum == 0.0)) {
         // no teacher in this row: nothing is read (the whole cluster leaves here)
         if (rank == 0) write_no_teacher(a, row);
         return;
@@ -401,17 +408,31 @@ __global__ void __launch_bounds__(kBwdThreads, 6) distill_topk_bwd_kernel(const 
     if (zero) return;
     __syncthreads();   // the piece is written; the listed columns follow
     if (mine) {
+        // A renormalised list's log normaliser is saved in 32 bits. Where they resolve less than 2^-21 of a weight it is
+        // taken again, from differences to the list's largest value.
+        float base = log_norm, norm = 1.0f;
+        if (fabsf(log_norm) >= 8.0f) {
+            base = -CUDART_INF_F;
+#pragma unroll 1
+            for (int k = 0; k < a.top_k; ++k)
+                if (column[k] >= 0) base = fmaxf(base, a.teacher[row * a.top_k + k]);
+            float sum = 0.0f;
+#pragma unroll 1
+            for (int k = 0; k < a.top_k; ++k)
+                if (column[k] >= 0) sum += expf(a.teacher[row * a.top_k + k] - base);
+            norm = 1.0f / sum;
+        }
         // a column that appears more than once: the first place writes for all, in list order
         float w = 0.0f;
         bool earlier = false;
         for (int k = 0; k < a.top_k; ++k) {
             if (column[k] == c) {
                 earlier |= k < tid;
-                w += expf(a.teacher[row * a.top_k + k] - log_norm);
+                w += expf(a.teacher[row * a.top_k + k] - base);
             }
         }
         const float q = ex2_approx(fmaf(listed - all_m, k2, -all_log * kLog2e));
-        if (!earlier) Vec<T>::store(map.out + c, g * (q - w));
+        if (!earlier) Vec<T>::store(map.out + c, g * (q - w * norm));
     }
 }
 

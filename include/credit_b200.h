@@ -383,7 +383,7 @@ int credit_token_logprobs_backward(const void* logits, int64_t row_stride, const
  *   - With tail = 1, when the student has nothing left outside the list, or the list sums to
  *     more than 1, the teacher is renormalised over the list.
  *   - Masked (-inf) logits under teacher mass give loss +inf and a finite gradient; a row of
- *     -inf only has no gradient; NaN or +inf in a row gives NaN.
+ *     -inf only has no gradient; NaN or +inf in a row, or at a used place of its list, gives NaN.
  * dlogits and its stride as in credit_token_logprobs_backward. */
 int credit_distill_topk_forward(const void* logits, int64_t row_stride, const int64_t* teacher_index,
                                 const float* teacher_logprob, int top_k, float* loss, float* stats,

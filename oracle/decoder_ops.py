@@ -152,8 +152,9 @@ def distill_topk_forward(logits, index, logprob, temperature=1.0, tail=True):
             continue
         values = torch.tensor([v for _, v in places], dtype=F64)
         mass = float(values.exp().sum())
+        log_mass = float(torch.logsumexp(values, 0)) if places else -math.inf    # also where mass leaves fp64's range
         stats[r, 0] = -math.inf
-        if not places or (not tail and mass == 0.0):
+        if not places or (not tail and log_mass == -math.inf):
             continue
         m, log_sum, d = (t[0] for t in _row_softmax(x[None], temperature))
         columns = torch.tensor([c for c, _ in places])
@@ -163,11 +164,11 @@ def distill_topk_forward(logits, index, logprob, temperature=1.0, tail=True):
         m2, log_sum2, _ = (t[0] for t in _row_softmax(outside[None], temperature))
         norm, rest = 0.0, 0.0
         if not tail:
-            norm = float(torch.logsumexp(values, 0))
+            norm = log_mass
         elif m2 == -math.inf or mass > 1.0:
-            if mass == 0.0:
+            if log_mass == -math.inf:
                 continue
-            norm = math.log(mass)
+            norm = log_mass
         else:
             rest = 1.0 - mass
         total = 0.0
