@@ -37,7 +37,6 @@ struct TopBuffer {
     static constexpr int kPlaces = 8 * THREADS;
     unsigned long long keys[kPlaces];
     unsigned int hist[256];
-    unsigned long long lowest;   // smallest kept key
     float group[kTopGroups][THREADS];   // maxima
     unsigned int floor[THREADS / 32];   // image of each warp's share of the threshold
     unsigned int differ[2];      // bits in which the keys differ (high, low word); zero between calls
@@ -85,10 +84,9 @@ __device__ __forceinline__ void find_digit(TopBuffer<THREADS>& t, int need) {
 }
 
 // Keeps the k largest of keys[0, n), n <= kPlaces (fewer when fewer are non-zero: zeros are
-// empty places), and returns the smallest of them (0 when there are fewer than k). All threads call
-// it behind a barrier; it ends with one, the number kept in t.fill.
+// empty places). All threads call it behind a barrier; it ends with one, the number kept in t.fill.
 template <int THREADS>
-__device__ __forceinline__ uint64_t keep_largest(TopBuffer<THREADS>& t, int n, int k) {
+__device__ __forceinline__ void keep_largest(TopBuffer<THREADS>& t, int n, int k) {
     constexpr int kPer = TopBuffer<THREADS>::kPlaces / THREADS;
     const int tid = threadIdx.x;
     uint64_t mine[kPer];
@@ -136,27 +134,19 @@ __device__ __forceinline__ uint64_t keep_largest(TopBuffer<THREADS>& t, int n, i
     } else if (n <= k) {
         threshold = 0;
     }
-    if (tid == 0) {
-        t.fill = 0;
-        t.lowest = ~0ull;
-    }
+    if (tid == 0) t.fill = 0;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        if (mine[j] != 0 && mine[j] >= threshold) {
-            t.keys[atomicAdd(&t.fill, 1)] = mine[j];
-            atomicMin(&t.lowest, static_cast<unsigned long long>(mine[j]));
-        }
-    }
+    for (int j = 0; j < kPer; ++j)
+        if (mine[j] != 0 && mine[j] >= threshold) t.keys[atomicAdd(&t.fill, 1)] = mine[j];
     if (tid == 0) t.differ[0] = t.differ[1] = 0;
     __syncthreads();
-    return t.fill < k ? 0 : t.lowest;
 }
 
 // The same, sorted descending: with one key a thread at most, the larger ones are counted for each, which is
-// its place; more go through the digits first. Returns the k-th (0 when there are fewer).
+// its place; more go through the digits first. The number kept is in t.fill.
 template <int THREADS>
-__device__ __noinline__ uint64_t rank_largest(TopBuffer<THREADS>& t, int n, int k) {
+__device__ __noinline__ void rank_largest(TopBuffer<THREADS>& t, int n, int k) {
     const int tid = threadIdx.x;
     if (n > THREADS) {
         keep_largest(t, n, k);
@@ -183,7 +173,6 @@ __device__ __noinline__ uint64_t rank_largest(TopBuffer<THREADS>& t, int n, int 
     if (mine != 0 && part == 0 && place < k) t.keys[place] = mine;
     if (tid == 0) t.fill = min(kept, k);
     __syncthreads();
-    return kept >= k ? t.keys[k - 1] : 0;
 }
 
 // The slow path: the same selection straight from the slice in global memory. Leaves at most k keys
