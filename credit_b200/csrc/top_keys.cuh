@@ -9,8 +9,12 @@
 // does not depend on the order in which threads append. NaN ranks above +inf, -0 equals +0, -inf is
 // never an element (its image lies under kLowestKey).
 //
-// A slice with more groups or elements at the threshold than there are places (thousands of ties) is searched by
-// the digit-by-digit selection straight from global memory, at most 8 more reads of it.
+// When more groups or elements reach the threshold than there are places, it is mostly one value that thousands of
+// elements share: a constant row, or a finite mask that leaves some warp fewer tokens than its share. Then the
+// elements above it compete, and those equal to it in the order of their columns until there are k: 592 x 131072 bf16
+// rows of -1e9 with 8 tokens left, k = 20, 70 us a call (ordinary rows 40 us; by the digits below 2627 us). Only a
+// slice with too many elements above it too is searched digit by digit straight from global memory, at most 9 more
+// reads of it.
 //
 // What was measured before this form, 4096 rows of 131072 bf16, k = 20 (164 us without alternatives): a running
 // threshold made exact after chunks 1, 4, 16 by all threads 270 us; kept by the warps without barriers 315 us: noting
@@ -225,6 +229,61 @@ __device__ __noinline__ void select_from_slice(const T* first, int start, int lo
     __syncthreads();
 }
 
+// The middle path: the elements above the bound `least` (an image), and when they are fewer than k the first ones
+// equal to it, at least k together, into keys[0, n). Returns n (more than kPlaces: too many, the keys are void). All
+// threads, behind a barrier; ends with one.
+template <typename T, int THREADS, int U>
+__device__ __noinline__ int collect_from_bound(const RowSpan<T> span, uint32_t least, int groups, int per_group, int k,
+                                               TopBuffer<THREADS>& t) {
+    constexpr int E = Vec<T>::kElems, kPlaces = TopBuffer<THREADS>::kPlaces, kStep = 4;
+    static_assert(kMaxTop + kStep * THREADS <= kPlaces, "fewer than k keys and all of a step fit");
+    const int tid = threadIdx.x;
+    auto offer = [&](float x, int offset) {
+        const int at = atomicAdd(&t.count, 1);
+        if (at < kPlaces) t.keys[at] = element_key(x, span.start + offset);
+    };
+    if (tid == 0) t.count = t.notes = 0;
+    __syncthreads();
+    if (tid < span.edges) {
+        const int offset = span.edge_offset(tid);
+        const float x = Vec<T>::load(span.first + offset);
+        if (ordered_image(x) > least) offer(x, offset);
+    }
+    for (int g = 0; g < groups; ++g)
+        if (ordered_image(t.group[g][tid]) > least) {
+            const int at = atomicAdd(&t.notes, 1);
+            if (at < kPlaces) t.noted[at] = g * THREADS + tid;
+        }
+    __syncthreads();
+    const int notes = t.notes, vectors = U * per_group;
+    if (notes > kPlaces) return notes;   // an element each at least
+    for (int i = tid; i < notes * vectors; i += THREADS) {
+        const int note = t.noted[i / vectors];
+        const int v = ((note / THREADS * per_group) * U + i % vectors) * THREADS + note % THREADS;
+        if (v >= span.nvec) continue;
+        float x[E];
+        Vec<T>::unpack(span.vectors()[v], x);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (ordered_image(x[j]) > least) offer(x[j], span.head + v * E + j);
+    }
+    __syncthreads();
+    int n = t.count;
+    __syncthreads();
+    for (int base = 0; base < span.local && n < k; base += kStep * THREADS) {
+#pragma unroll
+        for (int j = 0; j < kStep; ++j) {
+            const int i = base + j * THREADS + tid;
+            const float x = i < span.local ? Vec<T>::load(span.first + i) : -CUDART_INF_F;
+            if (ordered_image(x) == least) offer(x, i);
+        }
+        __syncthreads();
+        n = t.count;
+        __syncthreads();
+    }
+    return n;
+}
+
 // One CTA's groups while its slice streams by, in chunks of U vectors a thread.
 template <typename T, int THREADS, int U>
 struct TopCollector {
@@ -317,9 +376,13 @@ struct TopCollector {
         int n = t.count;
         if (overflow || n > kPlaces) {
             __syncthreads();
-            select_from_slice(span.first, span.start, span.local, k, t);
-            n = t.fill;
-            __syncthreads();
+            n = collect_from_bound<T, THREADS, U>(span, least, groups, per_group, k, t);
+            if (n > kPlaces) {
+                __syncthreads();
+                select_from_slice(span.first, span.start, span.local, k, t);
+                n = t.fill;
+                __syncthreads();
+            }
         }
         rank_largest(t, n, k);
     }
