@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
+constexpr int64_t kLongRowBytes = 224 * 1024;   // a row that takes larger CTAs when it has alternatives
 
 struct LogprobArgs {
     const void* logits;
@@ -305,11 +306,16 @@ int forward(const void* logits, int64_t ld, const int64_t* targets, float* logpr
     a.status = ctx.status;
     const bool top = top_k > 0;
     // Half as many threads a row let twice as many rows overlap, whose reductions, selections and ends are then hidden,
-    // once the rows fill the eight CTAs an SM that fit: bf16 8192 x 16384 67 -> 51 us, 8192 x 2048 45 -> 24, 4096 x 131072
-    // 169 -> 161; with 20 alternatives 8192 x 16384 135 -> 93, 8192 x 32768 169 -> 129, 4096 x 131072 203 / 206 (1184
-    // such rows 68 / 73). With fewer rows the CTAs with more loads in flight win (900 x 131072 43 us against 50, 300 x 131072 23 against 32), and
-    // so do those with more maxima to bound many alternatives by (64 of 4096 x 131072: 230 against 256).
-    const int threads = cluster == 1 && rows >= 8 * ctx.sm_count && top_k <= 32 ? kThreads / 2 : kThreads;
+    // once the rows fill the eight CTAs an SM that fit. 256 / 128 threads, us, one build, inputs changing: bf16 8192 x
+    // 2048 45.6 / 25.1, 8192 x 16384 68.3 / 52.8, 8192 x 32768 101.9 / 91.7; fewer rows: 300 x 131072 23.7 / 29.5, 900 x
+    // 65536 26.9 / 27.0. Longer rows hide them anyway; without alternatives the two are within 4 % there, either way (bf16
+    // 4096 x 131072 168 / 165, 2048 x 262144 167 / 168, 2400 x 122880 99 / 102; fp32 2048 x 131072 159 / 154, 4096 x 65536
+    // 154 / 158). With them the maxima of more threads bound a long row's alternatives closer. k = 20: bf16 8192 x 16384
+    // 137 / 95, 8192 x 32768 175 / 133, 3000 x 98304 133 / 131, 2400 x 122880 124 / 129, 1184 x 131072 66 / 71, 4096 x
+    // 131072 197 / 205; fp32 3000 x 49152 119 / 117, 2400 x 61440 117 / 125. k = 64: bf16 8192 x 32768 215 / 188, 4096 x
+    // 131072 230 / 256; k = 128: 8192 x 32768 324 / 1008 (too few maxima for so many).
+    const bool half = !top || (top_k <= 32 && cols * element_bytes(dtype) < kLongRowBytes);
+    const int threads = cluster == 1 && rows >= 8 * ctx.sm_count && half ? kThreads / 2 : kThreads;
     const void* func = dtype == CREDIT_BF16 ? forward_kernel<__nv_bfloat16>(entropy != nullptr, top, threads)
                                             : forward_kernel<float>(entropy != nullptr, top, threads);
     rc = prepare_kernel(ctx, func);
