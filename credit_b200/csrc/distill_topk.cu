@@ -11,7 +11,9 @@
 // its gradient to full precision; w_r is taken in 64 bits for the same reason.
 // A renormalised list may lie anywhere (raw logits): its weights are taken from differences to its largest value.
 // No reference kernel exists for this; the row pass is that of token_logprobs.cu and bound as it is: bf16 on one B200,
-// 2048 x 131072 with a list of 64 97 us = 5.5 TB/s (fp32 159 us = 6.8 TB/s), the gradient 173 us = 6.2 TB/s.
+// 2048 x 131072 with a list of 64 98 us = 5.5 TB/s replayed from a graph, 109 us = 4.9 TB/s in a long loop over changing
+// inputs; the gradient 179 us = 6.0 TB/s and 187 us. Shorter rows show what a row costs beside its logits (the list, its
+// marks, one warp's finish): 8192 x 16384 88 us = 3.1 TB/s.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

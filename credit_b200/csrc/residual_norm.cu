@@ -24,9 +24,10 @@ namespace {
 // thread, whose parameters (and, in the backward pass, sums over the rows) stay in registers. The rows come
 // through a ring of shared-memory stages filled by bulk copies, so the next rows are on their way while one is
 // reduced. A row step has one barrier. HBM bounds both directions (4 and 6 matrices move, some 10 and 26 flops an
-// element): bf16 on one B200, forward 16384 x 8192 168 us = 6.4 TB/s, backward 16384 x 4096 136 us = 5.9 TB/s, where three
-// stages of four inputs are what fits. Unaligned rows are bound by their instructions, one element at a time: fp32
-// backward 2049 x 5003 66 us = 3.7 TB/s.
+// element): bf16 on one B200, forward 16384 x 8192 168 us = 6.4 TB/s replayed from a graph, 189 us = 5.7 TB/s in a long
+// loop over changing inputs (without post norm and gate 190 us replayed); backward 16384 x 4096 136 us = 5.9 TB/s and
+// 154 us = 5.2 TB/s, where three stages of four inputs are what fits. Unaligned rows are bound by their instructions, one
+// element at a time: fp32 backward 2049 x 5003 66 us = 3.7 TB/s (loop 68), bf16 16384 x 5003 forward 242 us, backward 339.
 constexpr int kMaxRing = 8;
 
 template <typename T>

@@ -7,8 +7,9 @@
 // (src/workloads/softmax_logits_backward.cu:410).
 //
 // Both directions are bound by HBM, the forward pass with the exponential unit at two thirds beside it: bf16 on one
-// B200, 4096 x 131072 with entropy 161 us = 6.35 TB/s (1024 threads an SM, 128 or 256 a row; a chunk of four vectors
-// a thread with the next one in flight), with 20 alternatives 205 us; the gradient of 4096 x 65536 155 us = 6.7 TB/s. Eight rows of
+// B200, 4096 x 131072 with entropy 161 us = 6.35 TB/s replayed from a graph, 189 us = 5.4 TB/s in a long loop over changing
+// inputs (1024 threads an SM, 128 or 256 a row; a chunk of four vectors a thread with the next one in flight); with 20
+// alternatives 198-207 us, with 64 224-234 (replayed); the gradient of 4096 x 65536 155 us = 6.7 TB/s (loop 158). Eight rows of
 // 131072 with 20 alternatives take 10 us: latency of a selection in each CTA and one over the cluster.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -306,14 +307,14 @@ int forward(const void* logits, int64_t ld, const int64_t* targets, float* logpr
     a.status = ctx.status;
     const bool top = top_k > 0;
     // Half as many threads a row let twice as many rows overlap, whose reductions, selections and ends are then hidden,
-    // once the rows fill the eight CTAs an SM that fit. 256 / 128 threads, us, one build, inputs changing: bf16 8192 x
-    // 2048 45.6 / 25.1, 8192 x 16384 68.3 / 52.8, 8192 x 32768 101.9 / 91.7; fewer rows: 300 x 131072 23.7 / 29.5, 900 x
-    // 65536 26.9 / 27.0. Longer rows hide them anyway; without alternatives the two are within 4 % there, either way (bf16
-    // 4096 x 131072 168 / 165, 2048 x 262144 167 / 168, 2400 x 122880 99 / 102; fp32 2048 x 131072 159 / 154, 4096 x 65536
-    // 154 / 158). With them the maxima of more threads bound a long row's alternatives closer. k = 20: bf16 8192 x 16384
-    // 137 / 95, 8192 x 32768 175 / 133, 3000 x 98304 133 / 131, 2400 x 122880 124 / 129, 1184 x 131072 66 / 71, 4096 x
-    // 131072 197 / 205; fp32 3000 x 49152 119 / 117, 2400 x 61440 117 / 125. k = 64: bf16 8192 x 32768 215 / 188, 4096 x
-    // 131072 230 / 256; k = 128: 8192 x 32768 324 / 1008 (too few maxima for so many).
+    // once the rows fill the eight CTAs an SM that fit. 256 / 128 threads, us, one run of one build, inputs changing: bf16
+    // 8192 x 2048 45.7 / 25.1, 8192 x 16384 68.3 / 52.7, 8192 x 32768 101.9 / 91.8; fewer rows: 300 x 131072 23.4 / 29.5,
+    // 900 x 65536 26.8 / 26.7. Longer rows hide them anyway; without alternatives the two are within 6 % there, either way
+    // (bf16 4096 x 131072 169 / 170, 2048 x 262144 177 / 181; fp32 2048 x 131072 160 / 155, 2400 x 61440 93 / 99). With them
+    // the maxima of more threads bound a long row's alternatives closer. k = 20: bf16 8192 x 16384 137 / 95, 8192 x 32768
+    // 174 / 132, 3000 x 98304 128 / 127, 2400 x 122880 127 / 130, 4096 x 131072 207 / 221; fp32 3000 x 49152 118 / 117, 2400 x
+    // 61440 117 / 124. k = 64: bf16 8192 x 32768 223 / 192, 4096 x 131072 234 / 266; k = 128: 8192 x 32768 334 / 1033 (too few
+    // maxima for so many).
     const bool half = !top || (top_k <= 32 && cols * element_bytes(dtype) < kLongRowBytes);
     const int threads = cluster == 1 && rows >= 8 * ctx.sm_count && half ? kThreads / 2 : kThreads;
     const void* func = dtype == CREDIT_BF16 ? forward_kernel<__nv_bfloat16>(entropy != nullptr, top, threads)

@@ -62,7 +62,8 @@ inline int chunks_per_piece(int64_t rows, int64_t cols, int chunk_elems, int mos
 inline int row_slice(int64_t cols, int cluster) { return static_cast<int>(((cols + cluster - 1) / cluster + 63) / 64 * 64); }
 
 // CTAs per row of the kernels that reduce a row: the largest cluster that leaves all of them resident at once (`ctas`)
-// and slices of more than half a chunk. bf16, 131072 columns, 1 / 2 / 4 / 8 CTAs a row: token_logprobs with 100 rows
+// and slices of more than half of `chunk` columns, a bf16 chunk of the kernel for both types (so fp32 slices are a whole
+// one of theirs at least). bf16, 131072 columns, 1 / 2 / 4 / 8 CTAs a row: token_logprobs with 100 rows
 // 13.6 / 10.9 / 9.2 / 10.6 us, 300 rows 22.1 / 16.8 / 18.4 / 23.3, 400 rows 24.3 / 24.8 / 26.4 / 33.3; with
 // alternatives 200 rows 23.4 / 20.9 / 26.4 / 34.5, 300 rows 27.7 / 31.0 / 36.0 / 49.7; distill_topk with 256 rows
 // 27.6 / 20.8 / 19.3 / 21.7, 600 rows 41.0 / 42.3 / 42.0 / 49.1.

@@ -397,7 +397,7 @@ int credit_distill_topk_backward(const void* logits, int64_t row_stride, const i
 
 /* Host-buffer entry points ----------------------------------------------- */
 
-/* The workloads above on HOST data. Every matrix and vector argument named *_host is
+/* The row workloads on HOST data (the operators of the section before have no such form). Every matrix and vector argument named *_host is
  * host memory; `scratch` is caller-owned DEVICE memory (256-byte aligned) of at least
  * the matching *_host_scratch_bytes(). A matrix is streamed through the scratch in row
  * blocks on three streams: the upload of block k+1, the kernels of block k and the
