@@ -62,3 +62,28 @@ def test_lists_far_from_zero(native_lib, dtype, tail, offset, cluster):
     extra = ls.abs() + ls2.abs() + ((m - m2).abs() / temperature).nan_to_num(0.0, 0.0, 0.0)
     _within(grad, want, mag * U * (64 + 16 * far + 16 * extra[:, None]) + _rounding(dtype, want), "dlogits")
     assert N.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [True, False])
+@pytest.mark.parametrize("cluster", [1, 4])
+def test_nan_and_inf_at_a_used_place(native_lib, dtype, tail, cluster):
+    """NaN throughout such a row; the rows beside it, and the same values at unused places, are as they were."""
+    x, index, value = _inputs(dtype, 1003, 12, -2.0)
+    want_ins = (x.to(DEV), index.to(DEV), value.to(DEV))
+    value, index = value.clone(), index.clone()
+    value[0, 5], value[2, 0] = NAN, math.inf
+    value[3, 2], value[3, 3] = math.inf, NAN           # unused places
+    dloss = torch.ones(5, device=DEV)
+    results = []
+    for ins in (want_ins, (x.to(DEV), index.to(DEV), value.to(DEV))):
+        outs = _poisoned(L.allocate_outputs("distill_topk_forward", ins))
+        _launch("distill_topk_forward", ins, outs, cluster_size=cluster, tail=tail)
+        (grad,) = _poisoned(L.allocate_outputs("distill_topk_backward", ins))
+        _launch("distill_topk_backward", (*ins, outs[1], dloss), (grad,), tail=tail)
+        results.append((outs[0], grad))
+    (loss, grad), (got_loss, got_grad) = results
+    broken = torch.tensor([True, False, True, False, False], device=DEV)
+    assert bool(torch.isnan(got_loss[broken]).all()) and bool(torch.isnan(got_grad[broken]).all())
+    assert torch.equal(got_loss[~broken], loss[~broken]) and torch.equal(got_grad[~broken], grad[~broken])
+    assert N.device_status() == 0
