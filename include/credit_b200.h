@@ -398,8 +398,9 @@ int credit_distill_topk_backward(const void* logits, int64_t row_stride, const i
 /* Host-buffer entry points ----------------------------------------------- */
 
 /* The row workloads on HOST data (the operators of the section before have no such
- * form). Every matrix and vector argument named *_host is host memory; `scratch` is caller-owned DEVICE memory (256-byte aligned) of at least
- * the matching *_host_scratch_bytes(). A matrix is streamed through the scratch in row
+ * form). Every matrix and vector argument named *_host is host memory; `scratch` is
+ * caller-owned DEVICE memory (256-byte aligned) of at least the matching
+ * *_host_scratch_bytes(). A matrix is streamed through the scratch in row
  * blocks on three streams: the upload of block k+1, the kernels of block k and the
  * download of block k-1 overlap. More scratch than the minimum lets the blocks grow,
  * up to the whole matrix. Pinned host memory makes the copies asynchronous to each
